@@ -115,6 +115,15 @@ SIGNATURES = {
                               VP, VP]),
     'kfac_wire_unpack_sum_as': (I, [I, I, c_void_pp, c_i64_p, c_int_p,
                                     c_int_p, F, F, c_void_pp, I, VP]),
+    'kfac_embedding': (I, [I, VP, I64, I, VP, I, I64, I, I64, F, VP, VP]),
+    'kfac_token_order_workspace_bytes': (SZ, [I64, I64]),
+    'kfac_token_order': (I, [VP, I, I64, I64, I, I64, VP, VP, VP, SZ, VP]),
+    'kfac_embedding_grad_workspace_bytes': (SZ, [I64, I]),
+    'kfac_embedding_grad': (I, [I, VP, I, VP, VP, I64, I64, F, I, VP, VP, SZ,
+                                VP]),
+    'kfac_token_counts_workspace_bytes': (SZ, [I64]),
+    'kfac_token_counts': (I, [VP, I, I64, I64, I, I64, F, F, VP, VP, VP, SZ,
+                              VP]),
 }
 
 ERR_WORKSPACE = 3        # KFAC_ERR_WORKSPACE

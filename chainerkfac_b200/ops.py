@@ -787,3 +787,178 @@ def wire_unpack_sum(arrays, tri, wire_ptrs, select=None, scale=1.0,
 def wire_unpack(arrays, tri, wire, select=None, scale=1.0, ema_r=-1.0):
     wire_unpack_sum(arrays, tri, [wire.data_ptr()], select, scale, ema_r,
                     wire_dtype=wire.dtype)
+
+
+# -- token embeddings ---------------------------------------------------------
+# These check that their tensors share a device and run there, whichever device
+# is current; scratch comes from the caching allocator call by call, so calls on
+# several streams and captured graphs never share it.
+
+def _chk_rows(t, name, dtypes=WIRE_DTYPES):
+    if not t.is_cuda:
+        raise _lib.KfacLibraryError(
+            '%s must be a CUDA tensor: this package has no CPU path' % name)
+    if t.dtype not in dtypes:
+        raise TypeError('%s must be float32, float16 or bfloat16, got %s'
+                        % (name, t.dtype))
+    if not t.is_contiguous():
+        raise ValueError('%s must be contiguous' % name)
+
+
+def _chk_ids(ids):
+    if not ids.is_cuda:
+        raise _lib.KfacLibraryError(
+            'ids must be a CUDA tensor: this package has no CPU path')
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError('ids must be int64 or int32, got %s' % ids.dtype)
+    if not ids.is_contiguous():
+        raise ValueError('ids must be contiguous')
+
+
+def _chk_place(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError('%s is on %s, not on %s' % (name, t.device,
+                                                         device))
+
+
+def _chk_shape(t, shape, name):
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError('%s must be %s, got %s' % (
+            name, 'x'.join(str(v) for v in shape), tuple(t.shape)))
+
+
+def _scratch(nbytes, device):
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+def _ignore(label):
+    return (0, 0) if label is None else (1, int(label))
+
+
+def embedding(weight, ids, scale=1.0, ignore_label=None, out=None):
+    """out[..., :] = scale * weight[ids] for a (vocab, width) ``weight``
+    (float32, float16 or bfloat16; the product is rounded once) and int64 or
+    int32 ``ids`` of any shape.  Rows of ``ignore_label`` are zeros; an id
+    outside the vocabulary gives a row of NaN."""
+    _chk_rows(weight, 'weight')
+    _chk_ids(ids)
+    if weight.dim() != 2:
+        raise ValueError('weight must have two dimensions')
+    device = weight.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return embedding(weight, ids, scale, ignore_label, out)
+    vocab, width = weight.shape
+    shape = ids.shape + (width,)
+    if out is None:
+        out = torch.empty(shape, dtype=weight.dtype, device=device)
+    else:
+        _chk_rows(out, 'out', (weight.dtype,))
+        _chk_shape(out, shape, 'out')
+    _chk_place(device, ids=ids, out=out)
+    has, label = _ignore(ignore_label)
+    _lib.check(_lib.load().kfac_embedding(
+        WIRE_DTYPES[weight.dtype], weight.data_ptr(), vocab, width,
+        ids.data_ptr(), ids.element_size(), ids.numel(), has, label, scale,
+        out.data_ptr(), _stream()), 'kfac_embedding')
+    return out
+
+
+class TokenOrder(object):
+    """The positions of a batch's tokens, sorted by token (equal ones in their
+    order): what ``embedding_grad`` walks, made once however many gradients
+    are taken over the batch."""
+
+    def __init__(self, ids, vocab, ignore_label=None):
+        _chk_ids(ids)
+        self.device, self.vocab = ids.device, int(vocab)
+        self.count = ids.numel()
+        with torch.cuda.device(self.device):
+            lib = _lib.load()
+            self.keys, self.positions = torch.empty(
+                (2, self.count), dtype=torch.int32,
+                device=self.device).unbind(0)
+            ws = _scratch(lib.kfac_token_order_workspace_bytes(
+                self.count, self.vocab), self.device)
+            self.stream = _stream()
+            has, label = _ignore(ignore_label)
+            _lib.check(lib.kfac_token_order(
+                ids.data_ptr(), ids.element_size(), self.count, self.vocab,
+                has, label, self.keys.data_ptr(), self.positions.data_ptr(),
+                ws.data_ptr(), ws.numel(), self.stream), 'kfac_token_order')
+
+    def used_here(self):
+        """Keeps the sorted positions from being handed out again while the
+        current stream reads them, where that is another than theirs."""
+        if _stream() != self.stream:
+            self.keys.record_stream(torch.cuda.current_stream())
+
+
+def embedding_grad(gy, order, scale=1.0, out=None, accumulate=False):
+    """out[v, :] = scale * sum of ``gy``'s rows at the positions of token v,
+    for all tokens of ``order``'s vocabulary; with ``accumulate`` the sums are
+    added to ``out``.  ``gy``: (..., width), a row per token of ``order``.
+    The same inputs give the same bits."""
+    _chk_rows(gy, 'gy')
+    if gy.dim() < 1 or gy.shape[-1] < 1:
+        raise ValueError('gy must have rows')
+    width = gy.shape[-1]
+    if gy.numel() != order.count * width:
+        raise ValueError('gy must have a row for each of the %d tokens, got %s'
+                         % (order.count, tuple(gy.shape)))
+    device = gy.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return embedding_grad(gy, order, scale, out, accumulate)
+    shape = (order.vocab, width)
+    if out is None:
+        if accumulate:
+            raise ValueError('accumulate needs an existing `out`')
+        out = torch.empty(shape, dtype=gy.dtype, device=device)
+    else:
+        _chk_rows(out, 'out', (gy.dtype,))
+        _chk_shape(out, shape, 'out')
+    _chk_place(device, order=order, out=out)
+    lib = _lib.load()
+    ws = _scratch(lib.kfac_embedding_grad_workspace_bytes(order.count, width),
+                  device)
+    order.used_here()
+    _lib.check(lib.kfac_embedding_grad(
+        WIRE_DTYPES[gy.dtype], gy.data_ptr(), width, order.keys.data_ptr(),
+        order.positions.data_ptr(), order.count, order.vocab, scale,
+        int(bool(accumulate)), out.data_ptr(), ws.data_ptr(), ws.numel(),
+        _stream()), 'kfac_embedding_grad')
+    return out
+
+
+def token_counts(ids, vocab, ignore_label=None, alpha=1.0, beta=0.0, out=None,
+                 mean=None):
+    """out[v] = alpha * (how often token v occurs in ``ids``) + beta * out[v]
+    (float32); ``mean``, one element, gets the mean of the counts the same
+    way."""
+    _chk_ids(ids)
+    device = ids.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return token_counts(ids, vocab, ignore_label, alpha, beta, out,
+                                mean)
+    if out is None:
+        if beta != 0.0:
+            raise ValueError('beta != 0 needs an existing `out`')
+        out = torch.empty(vocab, dtype=torch.float32, device=device)
+    _chk(out, 'out')
+    _chk_shape(out, (vocab,), 'out')
+    if mean is not None:
+        _chk(mean, 'mean')
+        if mean.numel() != 1:
+            raise ValueError('mean must have one element')
+    _chk_place(device, out=out, mean=mean)
+    lib = _lib.load()
+    ws = _scratch(lib.kfac_token_counts_workspace_bytes(vocab), device)
+    has, label = _ignore(ignore_label)
+    _lib.check(lib.kfac_token_counts(
+        ids.data_ptr(), ids.element_size(), ids.numel(), vocab, has, label,
+        alpha, beta, out.data_ptr(), _p(mean), ws.data_ptr(), ws.numel(),
+        _stream()), 'kfac_token_counts')
+    return out

@@ -499,6 +499,50 @@ int kfac_wire_unpack_sum_as(int wire_dtype, int n_arrays, float* const* arrays,
                             const void* const* wires, int n_wires,
                             void* stream);
 
+/* ---------------------------------------------------------- token embeddings
+ * Rows of an embedding's weight (vocab x width) by token, and the gradient of
+ * that weight.  Elements (weight, out, gy) are fp32, fp16 or bf16, `dtype`
+ * numbered as the wire types above; sums are formed in fp32 and rounded once.
+ * Matrices are row-major and dense, tokens 4- or 8-byte integers (`id_bytes`),
+ * fewer than 2^31 - 4096 of them.  A token equal to `ignore` (has_ignore != 0)
+ * has no row: zeros in a lookup, nothing in a gradient or a count.  Neither
+ * has one outside 0 .. vocab - 1: NaN in a lookup, nothing elsewhere.
+ */
+
+/* out[i] = scale * weight[ids[i]], n rows. */
+int kfac_embedding(int dtype, const void* weight, int64_t vocab, int width,
+                   const void* ids, int id_bytes, int64_t n, int has_ignore,
+                   int64_t ignore, float scale, void* out, void* stream);
+
+/* Tokens in ascending order, equal ones in the order of their positions:
+ * keys[j] (vocab for a token without a row: those come last) and
+ * positions[j], n of each.  Passes of a radix sort; two for vocabularies below
+ * 2^18. */
+size_t kfac_token_order_workspace_bytes(int64_t n, int64_t vocab);
+int kfac_token_order(const void* ids, int id_bytes, int64_t n, int64_t vocab,
+                     int has_ignore, int64_t ignore, int* keys, int* positions,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[v] = scale * sum of gy[i] over the positions i of token v, in an order
+ * that depends on the tokens alone (same inputs, same bits); rows of other
+ * tokens are cleared.  accumulate != 0: added to `out`, whose other rows are
+ * left as they are.  `keys` / `positions`: of kfac_token_order. */
+size_t kfac_embedding_grad_workspace_bytes(int64_t n, int width);
+int kfac_embedding_grad(int dtype, const void* gy, int width, const int* keys,
+                        const int* positions, int64_t n, int64_t vocab,
+                        float scale, int accumulate, void* out,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* out[v] = alpha * (how often v occurs) + beta * out[v] for all `vocab`
+ * tokens: the diagonal of the input factor of an embedding, which is a fully
+ * connected layer on rows with a single one.  mean (or NULL): one float, the
+ * mean of the counts the same way. */
+size_t kfac_token_counts_workspace_bytes(int64_t vocab);
+int kfac_token_counts(const void* ids, int id_bytes, int64_t n, int64_t vocab,
+                      int has_ignore, int64_t ignore, float alpha, float beta,
+                      float* out, float* mean, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

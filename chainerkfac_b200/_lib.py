@@ -121,6 +121,10 @@ SIGNATURES = {
     'kfac_embedding_grad_workspace_bytes': (SZ, [I64, I]),
     'kfac_embedding_grad': (I, [I, VP, I, VP, VP, I64, I64, F, I, VP, VP, SZ,
                                 VP]),
+    'kfac_orthogonalize_workspace_bytes': (SZ, [I, c_int_p, c_int_p]),
+    'kfac_orthogonalize': (I, [I, I, c_int_p, c_int_p, c_void_pp, c_void_pp,
+                               c_void_pp, c_float_p, I, c_float_p, F, F, F,
+                               VP, SZ, VP]),
     'kfac_token_counts_workspace_bytes': (SZ, [I64]),
     'kfac_token_counts': (I, [VP, I, I64, I64, I, I64, F, F, VP, VP, VP, SZ,
                               VP]),

@@ -58,6 +58,9 @@ int ring_alloc(size_t bytes, void** out);
 // Status word of the inverse's diagonal kernel (inverse.cu).
 int diag_status_read(int* out);
 
+// Status word of the orthogonalisation's products (ortho.cu).
+int ortho_status_read(int* out);
+
 // Number of streaming multiprocessors of the current device (cached).
 int sm_count();
 

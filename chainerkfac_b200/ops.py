@@ -962,3 +962,88 @@ def token_counts(ids, vocab, ignore_label=None, alpha=1.0, beta=0.0, out=None,
         alpha, beta, out.data_ptr(), _p(mean), ws.data_ptr(), ws.numel(),
         _stream()), 'kfac_token_counts')
     return out
+
+
+# -- orthogonalised updates ---------------------------------------------------
+
+# a, b, c of X = a X + (b A + c A A) X: five steps take singular values between
+# 1e-3 and 1 to between 0.7 and 1.2
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def _coefficients(coefficients, steps):
+    rows = list(coefficients)
+    if rows and not hasattr(rows[0], '__len__'):
+        rows = [rows] * steps
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError('coefficients must be three numbers, or three for '
+                         'each of the %d steps' % steps)
+    return _lib.float_array([v for r in rows for v in r])
+
+
+def orthogonalize(xs, outs=None, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7,
+                  scale=1.0, params=None, lr=0.0, decay=0.0):
+    """Newton-Schulz orthogonalisation of updates: X = x / (|x|_F + eps), then
+    ``steps`` times X = a X + (b A + c A A) X with A = X X^T, for the three
+    ``coefficients`` (or three for each step).  Returns scale * X.
+
+    ``xs``: a tensor or a list (float32, float16 or bfloat16; the first
+    dimension against all others: a convolution's weight is a matrix of
+    filters); a list goes in one row of launches per type.  ``outs``: where to,
+    which may be ``xs``; ``scale``: a number, or one for each.  With weights
+    ``params`` (of the same types)
+    param = (1 - lr * decay) * param - lr * scale * X in the last product's
+    epilogue; only ``outs`` that are given are then written."""
+    if isinstance(xs, torch.Tensor):
+        got = orthogonalize([xs], None if outs is None else [outs], steps,
+                            coefficients, eps, [scale],
+                            None if params is None else [params], lr, decay)
+        return got[0]
+    xs = list(xs)
+    count = len(xs)
+    scales = list(scale) if hasattr(scale, '__len__') else [scale] * count
+    outs = [None] * count if outs is None else list(outs)
+    weights = [None] * count if params is None else list(params)
+    if not len(scales) == len(outs) == len(weights) == count:
+        raise ValueError('%d matrices, %d outputs, %d scales, %d weights' % (
+            count, len(outs), len(scales), len(weights)))
+    if not 1 <= steps <= 64:
+        raise ValueError('steps must be 1 to 64, got %d' % steps)
+    coef = _coefficients(coefficients, steps)
+    if not count:
+        return outs
+    device = xs[0].device
+    groups = {}
+    for i, (x, out, w) in enumerate(zip(xs, outs, weights)):
+        _chk_rows(x, 'x')
+        if x.dim() < 2 or x.numel() == 0:
+            raise ValueError('x must be a matrix, got %s' % (tuple(x.shape),))
+        for t, name in ((out, 'out'), (w, 'param')):
+            if t is not None:
+                _chk_rows(t, name, (x.dtype,))
+                _chk_shape(t, x.shape, name)
+        _chk_place(device, x=x, out=out, param=w)
+        groups.setdefault(x.dtype, []).append(i)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return orthogonalize(xs, outs, steps, coefficients, eps, scales,
+                                 params, lr, decay)
+    lib = _lib.load()
+    for dtype, idx in groups.items():
+        part = [xs[i] for i in idx]
+        rows = _lib.int_array([x.shape[0] for x in part])
+        cols = _lib.int_array([x.numel() // x.shape[0] for x in part])
+        for i in idx:
+            if outs[i] is None and weights[i] is None:
+                outs[i] = torch.empty_like(xs[i])
+        ws = _scratch(lib.kfac_orthogonalize_workspace_bytes(
+            len(idx), rows, cols), device)
+        _lib.check(lib.kfac_orthogonalize(
+            WIRE_DTYPES[dtype], len(idx), rows, cols,
+            _lib.ptr_array([x.data_ptr() for x in part]),
+            _lib.ptr_array([_p(outs[i]) for i in idx]),
+            _lib.ptr_array([_p(weights[i]) for i in idx]),
+            _lib.float_array([scales[i] for i in idx]), steps, coef, eps, lr,
+            decay, ws.data_ptr(), ws.numel(), _stream()),
+            'kfac_orthogonalize')
+    return outs

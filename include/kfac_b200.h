@@ -543,6 +543,29 @@ int kfac_token_counts(const void* ids, int id_bytes, int64_t n, int64_t vocab,
                       float* out, float* mean, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------ orthogonalised updates
+ * Newton-Schulz products of `count` matrices (rows[i] x cols[i], dense,
+ * row-major, elements as in the embeddings' calls), in one row of launches for
+ * up to 40 of them: X = x / (|x|_F + eps), then for each of `steps` (1 .. 64)
+ * rows (a, b, c) of `coefficients`
+ *     X = a X + (b A + c A A) X,   A = X X^T
+ * (X^T X and products from the right where rows exceed cols: the same values).
+ * out[i] = scale[i] * X, and with a weight, param[i] of the same type,
+ *     param = (1 - lr * decay) * param - lr * scale * X.
+ * Either may be NULL, as arrays or element by element; out[i] may be x[i].
+ * fp32 products carry 22 bits of their operands; for 16-bit matrices A and the
+ * polynomial carry 11.  An X with entries of 8 and more, or values that are
+ * not finite, give NaN.  Pointer, size and coefficient arrays are host arrays
+ * read during the call. */
+size_t kfac_orthogonalize_workspace_bytes(int count, const int* rows,
+                                          const int* cols);
+int kfac_orthogonalize(int dtype, int count, const int* rows, const int* cols,
+                       const void* const* x, void* const* out,
+                       void* const* param, const float* scale, int steps,
+                       const float* coefficients, float eps, float lr,
+                       float decay, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

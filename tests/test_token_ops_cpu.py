@@ -75,3 +75,60 @@ def test_workspaces_of_the_sort_and_the_gradient(lib):
     for n, width in ((1, 1), (100, 33), (70000, 2048), (2 ** 31 - 5000, 8)):
         need = lib.kfac_embedding_grad_workspace_bytes(n, width)
         assert 8 * width <= need <= 2 * 4 * (width + 3) * (n // 8 + 1)
+
+
+def ortho(lib, **k):
+    import numpy as np
+    from chainerkfac_b200 import _lib
+    a = {**dict(dtype=0, rows=[4], cols=[6], x=[4096], out=[8192], param=None,
+                scale=[1.0], steps=2, coef=[3.0, -4.0, 2.0] * 2, eps=1e-7,
+                lr=0.0, decay=0.0, ws=4096, nbytes=1 << 40), **k}
+    ptrs = lambda v: None if v is None else _lib.ptr_array(v)
+    return lib.kfac_orthogonalize(
+        a['dtype'], a.get('count', len(a['rows'])), _lib.int_array(a['rows']),
+        _lib.int_array(a['cols']), ptrs(a['x']), ptrs(a['out']),
+        ptrs(a['param']), _lib.float_array(a['scale']), a['steps'],
+        _lib.float_array(a['coef']), a['eps'], a['lr'], a['decay'],
+        ctypes.c_void_p(a['ws']), a['nbytes'], None)
+
+
+def test_orthogonalize_calls_are_checked(lib):
+    for bad in (dict(dtype=5), dict(rows=[0]), dict(cols=[-1]),
+                dict(rows=[2 ** 20 + 1]), dict(steps=0), dict(steps=65),
+                dict(eps=-1.0), dict(eps=float('nan')), dict(x=None),
+                dict(x=[None]), dict(out=None), dict(out=[None]),
+                dict(out=[None], param=[None]), dict(count=-1)):
+        assert ortho(lib, **bad) == 1, bad
+        assert 'orthogonalize' in message(lib)
+    assert ortho(lib, nbytes=64) == 3 and ortho(lib, ws=None) == 3
+    assert ortho(lib, rows=[], cols=[], x=[], out=[], scale=[]) == 0
+
+
+def test_workspace_of_an_orthogonalisation(lib):
+    """Two places of X, A and the polynomial, four bytes an element, rows of
+    whole 16-byte words."""
+    from chainerkfac_b200 import _lib
+
+    def need(*shapes):
+        return lib.kfac_orthogonalize_workspace_bytes(
+            len(shapes), _lib.int_array([s[0] for s in shapes]),
+            _lib.int_array([s[1] for s in shapes]))
+    for r, c in ((1, 1), (64, 147), (1000, 24), (4096, 4096)):
+        small = min(r, c)
+        least = 4 * (2 * r * c + 2 * small * small)
+        assert least <= need((r, c)) <= \
+            least + 4 * (2 * r * 8 + 2 * small * 8) + 8192
+    assert need((64, 64), (300, 20)) >= need((64, 64)) + need((300, 20)) - 512
+    assert need() == 0 and need((0, 4)) == 0
+
+
+def test_orthogonalize_refuses_what_is_not_a_matrix():
+    from chainerkfac_b200 import _lib, ops
+    x = torch.zeros(3, 4)
+    with pytest.raises(_lib.KfacLibraryError, match='CUDA tensor'):
+        ops.orthogonalize(x)
+    for bad in (dict(steps=0), dict(steps=65), dict(coefficients=(1.0, 2.0)),
+                dict(coefficients=[(1.0, 2.0, 3.0)] * 4), dict(scale=[1.0] * 2)):
+        with pytest.raises(ValueError):
+            ops.orthogonalize([x], **bad)
+    assert ops.orthogonalize([]) == []

@@ -175,30 +175,59 @@ struct EpiPlanes {
   float alpha, beta, diag;
   int terms;
   bool poly;
-  __device__ __forceinline__ void store(const PlaneProblem& g, const PlaneTile& t,
-                                        float (&v)[64], bool mirror) const {
+  __device__ __forceinline__ void store(const PlaneFields& g, const PlaneTile& t,
+                                        float (&v)[32], bool mirror) const {
 #pragma unroll
-    for (int i = 0; i < 64; ++i) v[i] *= alpha;
+    for (int i = 0; i < 32; ++i) v[i] *= alpha * g.gain;
     if (poly) {
-      const int r = t.r0 + t.lane;
-      const __half* p = g.add.p + (long long)r * g.add.ld + t.c0;
-      for (int term = 0; term < terms; ++term, p += g.add.plane) {
+      // `add` in the registers' order, by way of shared memory
+      const int j = t.lane & 3, r = t.lane >> 2;
+      const unsigned piece = smem_u32(t.piece);
+      const __half* p = g.add.p + (long long)(t.r0 + r) * g.add.ld + t.c0 + 8 * j;
+      const bool in = t.c0 + 8 * j < g.N;
+      uint4 w[2][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (r >= g.M || t.c0 + 8 * j >= g.N) continue;
-          const uint4 w = *reinterpret_cast<const uint4*>(p + 8 * j);
-          const unsigned u[4] = {w.x, w.y, w.z, w.w};
+      for (int term = 0; term < 2; ++term)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[term][i] = make_uint4(0, 0, 0, 0);
+          if (term < terms && in && t.r0 + r + 8 * i < g.M)
+            w[term][i] = *reinterpret_cast<const uint4*>(
+                p + (term ? g.add.plane : 0) + 8LL * i * g.add.ld);
+        }
+      __syncwarp();
+#pragma unroll
+      for (int term = 0; term < 2; ++term)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                       ::"r"(piece + 2048 * term + 512 * i + row64_off(r, j)),
+                         "r"(w[term][i].x), "r"(w[term][i].y), "r"(w[term][i].z),
+                         "r"(w[term][i].w)
+                       : "memory");
+      __syncwarp();
+#pragma unroll
+      for (int term = 0; term < 2; ++term)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          unsigned x[4];                 // rows' eighths
+          ld_matrix(piece + 2048 * term + row64_off(t.lane, k), x[0], x[1], x[2], x[3]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
-            v[8 * j + 2 * e] = fmaf(beta, x.x, v[8 * j + 2 * e]);
-            v[8 * j + 2 * e + 1] = fmaf(beta, x.y, v[8 * j + 2 * e + 1]);
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&x[e]));
+            const int at = 16 * (e >> 1) + 4 * k + 2 * (e & 1);
+            v[at] = fmaf(beta, y.x, v[at]);
+            v[at + 1] = fmaf(beta, y.y, v[at + 1]);
           }
         }
-      }
+      // (rows and columns past the matrix: of no matter)
+      if (t.r0 == t.c0) {
+        const int d = 2 * (t.lane & 3) - (t.lane >> 2);
 #pragma unroll
-      for (int i = 0; i < 64; ++i)
-        if (r == t.c0 + i) v[i] += diag;
+        for (int i = 0; i < 32; ++i)
+          if (16 * (i >> 4) + 8 * ((i >> 1) & 1) - 8 * ((i >> 2) & 3) - (i & 1) == d)
+            v[i] += diag;
+      }
     }
     pl_store_planes(t, g.out, v, g.M, g.N, terms, mirror);
   }
@@ -208,40 +237,84 @@ struct EpiPlanes {
 template <typename T>
 struct EpiLast {
   float alpha, keep, lr;
-  __device__ __forceinline__ void store(const PlaneProblem& g, const PlaneTile& t,
-                                        float (&v)[64], bool) const {
-    float* const piece = reinterpret_cast<float*>(t.piece);
+
+  // 32 x 32 values as rows of 128 bytes in shared memory, 16-byte words turned by the
+  // row: what a lane reads back is a column, or a word, of a row.
+  static __device__ __forceinline__ unsigned at(unsigned piece, int row, int word) {
+    return piece + row * 128 + ((word ^ (row & 7)) << 4);
+  }
+
+  __device__ __forceinline__ void store(const PlaneFields& g, const PlaneTile& t,
+                                        float (&v)[32], bool) const {
+    const unsigned piece = smem_u32(t.piece);
     T* const dst = static_cast<T*>(g.dst);
     T* const param = static_cast<T*>(g.param);
-    const float a = alpha * g.scale;
+    const float a = alpha * g.gain * g.scale;
+    const int lane = t.lane, N = g.N, rows = g.M - t.r0;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      __syncwarp();
+    for (int i = 0; i < 32; ++i) v[i] *= a;
+    __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        piece[t.lane * 32 + (i ^ t.lane)] = a * v[32 * half + i];
-      __syncwarp();
-      const int c = t.c0 + 32 * half + t.lane;
-      const int rows = c < g.N ? min(32, g.M - t.r0) : 0;
-      const long long at = (long long)t.r0 * g.N + c;
-#pragma unroll 1
-      for (int r = 0; r < 32; r += 8) {
-        float w[8], x[8];
+    for (int i = 0; i < 32; i += 2) {
+      const int row = 16 * (i >> 4) + 8 * ((i >> 1) & 1) + (lane >> 2);
+      asm volatile("st.shared.v2.f32 [%0], {%1, %2};"
+                   ::"r"(at(piece, row, 2 * ((i >> 2) & 3) + ((lane & 3) >> 1)) +
+                         8 * (lane & 1)),
+                     "f"(v[i]), "f"(v[i + 1])
+                   : "memory");
+    }
+    __syncwarp();
+    constexpr int W = 16 / sizeof(T);      // values of a 16-byte word
+    const bool words =
+        N % W == 0 && ((reinterpret_cast<uintptr_t>(dst) |
+                        reinterpret_cast<uintptr_t>(param)) & 15) == 0;
+    if (words) {
+      struct alignas(16) Word { T x[W]; };
+      constexpr int L = 32 / W, R = 32 / L;          // lanes of a row, rows at a time
+      const int c = t.c0 + W * (lane % L), r = lane / L;
+      if (c >= N) return;
+      const long long first = (long long)(t.r0 + r) * N + c, step = (long long)R * N;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          x[u] = piece[(r + u) * 32 + (t.lane ^ (r + u))];
-          w[u] = param != nullptr && r + u < rows
-                     ? as_float(param[at + (long long)(r + u) * g.N]) : 0.f;
+      for (int i = 0; i < 32 / R; ++i) {
+        if (r + R * i >= rows) break;
+        float x[W];
+#pragma unroll
+        for (int k = 0; k < W / 4; ++k)
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(x[4 * k]), "=f"(x[4 * k + 1]), "=f"(x[4 * k + 2]),
+                         "=f"(x[4 * k + 3])
+                       : "r"(at(piece, r + R * i, W / 4 * (lane % L) + k))
+                       : "memory");
+        Word o;
+        if (dst != nullptr) {
+#pragma unroll
+          for (int e = 0; e < W; ++e) o.x[e] = from_float<T>(x[e]);
+          *reinterpret_cast<Word*>(dst + first + step * i) = o;
         }
+        if (param != nullptr) {
+          o = *reinterpret_cast<const Word*>(param + first + step * i);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          if (r + u >= rows) continue;
-          if (dst != nullptr) dst[at + (long long)(r + u) * g.N] = from_float<T>(x[u]);
-          if (param != nullptr)
-            param[at + (long long)(r + u) * g.N] =
-                from_float<T>(fmaf(keep, w[u], -lr * x[u]));
+          for (int e = 0; e < W; ++e)
+            o.x[e] = from_float<T>(fmaf(keep, as_float(o.x[e]), -lr * x[e]));
+          *reinterpret_cast<Word*>(param + first + step * i) = o;
         }
       }
+      return;
+    }
+    const int c = t.c0 + lane;
+    if (c >= N) return;
+    const long long first = (long long)t.r0 * N + c;
+#pragma unroll 4
+    for (int i = 0; i < min(rows, 32); ++i) {
+      float x;
+      asm volatile("ld.shared.f32 %0, [%1];"
+                   : "=f"(x)
+                   : "r"(at(piece, i, lane >> 2) + 4 * (lane & 3))
+                   : "memory");
+      const long long k = first + (long long)i * N;
+      if (dst != nullptr) dst[k] = from_float<T>(x);
+      if (param != nullptr)
+        param[k] = from_float<T>(fmaf(keep, as_float(param[k]), -lr * x));
     }
   }
 };
@@ -302,7 +375,7 @@ struct Call {
 };
 
 template <int N, typename T>
-int launch_last(const PlaneLaunch<N>& l, const Call& c, cudaStream_t st) {
+int launch_last(PlaneLaunch<N>& l, const Call& c, cudaStream_t st) {
   const EpiLast<T> epi = {exp2f(-(kXExp + kAExp)), 1.f - c.lr * c.decay, c.lr};
   return plane_launch("ortho last product", l, epi, true, st);
 }
@@ -356,7 +429,7 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
     const Shape& m = s[i];
     const bool tall = m.rows > m.cols;
     const int r = m.small;
-    PlaneProblem g = {};
+    PlaneFields g = {};
     g.scale = c.scale[first + i];
     g.dst = c.out != nullptr ? c.out[first + i] : nullptr;
     g.param = c.param != nullptr ? c.param[first + i] : nullptr;
@@ -370,9 +443,9 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
         (rc = plane_map(&b, m.b, r, r, false)) != KFAC_OK)
       return rc;
     for (int k = 0; k < 2; ++k) {
-      PlaneProblem& p = gram[k].p[i];
+      gram[k].p[i].ma = gram[k].p[i].mb = tall ? down[k] : along[k];
+      PlaneFields& p = gram[k].p[i].f;
       p = g;
-      p.ma = p.mb = tall ? down[k] : along[k];
       p.a_mn = p.b_mn = tall;
       p.M = p.N = r;
       p.K = tall ? m.rows : m.cols;
@@ -380,21 +453,21 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
       // (of X for the product with itself one term, where A has one)
       p.ta = p.tb = terms;
       p.out = m.a;
-      PlaneProblem& q = apply[k].p[i];
+      apply[k].p[i].ma = tall ? along[k] : b;
+      apply[k].p[i].mb = tall ? b : down[k];
+      PlaneFields& q = apply[k].p[i].f;
       q = g;
       q.M = m.rows;
       q.N = m.cols;
       q.K = r;
-      q.ma = tall ? along[k] : b;
-      q.mb = tall ? b : down[k];
       q.b_mn = !tall;
       q.ta = tall ? 2 : terms;
       q.tb = tall ? terms : 2;
       q.out = m.x[k ^ 1];
     }
-    PlaneProblem& p = poly.p[i];
+    poly.p[i].ma = poly.p[i].mb = a;
+    PlaneFields& p = poly.p[i].f;
     p = g;
-    p.ma = p.mb = a;
     p.M = p.N = p.K = r;
     p.lower = p.same = 1;
     p.ta = p.tb = terms;

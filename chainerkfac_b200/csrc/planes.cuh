@@ -4,14 +4,23 @@
 // with two on both sides C = hi*hi + (hi*lo + lo*hi), the cross terms in an
 // accumulator of their own: 22 significant bits.
 //
-// Tiles of 128 x 128, k-blocks of 64: TMA lays both operands out as the MMAs read
-// them, whether k runs along the rows or down the columns of the planes, and fills
-// zeros past the edges, so any size goes without a copy.  One CTA an SM walks over
-// the tiles: warp 0 issues the loads, warp 1 the MMAs, eight warps take the
+// Tiles of 256 x 256 by pairs of CTAs (cta_group::2: each holds 128 rows of A and of
+// C, and half of B's rows), k-blocks of 64: TMA lays both operands out as the MMAs
+// read them, whether k runs along the rows or down the columns of the planes, and
+// fills zeros past the edges, so any size goes without a copy.  In each CTA warp 0
+// issues the loads and, in the first of a pair, warp 1 the MMAs; eight warps take the
 // accumulators, which are there twice, out of tensor memory while the MMAs go on in
-// the other pair.  The tensor core adds with truncation, so a sum of two-term
-// products is cut into segments of 512 k that add up in registers, rounded to
-// nearest.
+// the other one.
+//
+// The tensor core adds with truncation, so a long sum comes out too small by what
+// its number of additions makes: a sum of two-term products is cut every PL_SEGMENT
+// k-blocks and the segments are added in registers, rounded to nearest; within a
+// k-block the cross terms, 2^-11 of the others, go first, when the accumulator is
+// small.
+//
+// Launches with fewer tiles than the GPU has room for share the sum of a tile among
+// up to eight pairs of a cluster, which hand each other their parts through
+// distributed shared memory, added in the order of k.
 //
 // Every barrier wait is bounded; a wait that runs out raises the status word.
 #pragma once
@@ -19,6 +28,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 
 #include "gemm_simt.cuh"
@@ -29,18 +39,24 @@ namespace kfac {
 // Status word of the bounded waits, one in each source file that has products.
 static __device__ int g_plane_status = 0;
 
-constexpr int PL_BM = 128;                   // tile sides
+constexpr int PL_TILE = 256;                 // tile sides
+constexpr int PL_ROWS = 128;                 // rows of a CTA's part of A, B and C
 constexpr int PL_BK = 64;                    // k of a stage: 128 bytes of fp16
-constexpr int PL_TERM = PL_BM * PL_BK * 2;   // bytes of one term of an operand tile
+constexpr int PL_TERM = PL_ROWS * PL_BK * 2; // bytes of one term of such a part
 constexpr int PL_STAGE_BYTES = 12 * PL_TERM; // 192 KB of stages, 2 to 4 terms each
 constexpr int PL_STAGES_MAX = 6;
-constexpr int PL_SEGMENT = 8;                // k-blocks of an accumulator's sum
+// k-blocks of an accumulator's sum.  4096 x 4096, five steps: 4.9 ms and an error of
+// 0.9e-6 with one, 3.9 ms and 1.9e-6 with two, 3.7 ms and 3.7e-6 with four: of one, a
+// segment is in the tensor cores for less time than it takes to read.
+constexpr int PL_SEGMENT = 2;
+constexpr int PL_SPLIT_MAX = 8;              // pairs that share a tile
 constexpr int PL_EPI_WARPS = 8;
-constexpr int PL_THREADS = 32 * (2 + PL_EPI_WARPS);
+constexpr int PL_THREADS = 32 * (4 + PL_EPI_WARPS);
 constexpr int PL_PIECE = 4096;               // bytes of a warp's staging
 constexpr int PL_SMEM =
     PL_STAGE_BYTES + PL_EPI_WARPS * PL_PIECE + 1024 /* control */ + 1024 /* align */;
-constexpr int PL_COLS = 512;                 // tensor memory: 2 x (main, cross)
+constexpr int PL_COLS = 512;                 // tensor memory: two accumulators
+static_assert(PL_ROWS * PL_TILE * 4 <= PL_STAGE_BYTES, "parts of a shared sum");
 
 // A pair of planes.
 struct Planes {
@@ -49,8 +65,8 @@ struct Planes {
   int ld;                // elements of a row, a multiple of 8
 };
 
-struct alignas(64) PlaneProblem {
-  CUtensorMap ma, mb;
+// What the warps of a launch read of a problem, copied to registers for a tile.
+struct PlaneFields {
   int M, N, K;
   int tiles_n, tile_begin;
   int lower;             // square and symmetric: tiles on and below the diagonal
@@ -60,8 +76,14 @@ struct alignas(64) PlaneProblem {
   Planes out;            // of the result (not used by every epilogue)
   Planes add;
   float scale;
+  float gain;            // makes up for what the sums lose (plane_gain)
   void* dst;
   void* param;
+};
+
+struct alignas(64) PlaneProblem {
+  CUtensorMap ma, mb;
+  PlaneFields f;
 };
 
 template <int N>
@@ -70,6 +92,7 @@ struct PlaneLaunch {
   int n;
   int tiles;
   int terms;             // of both operands
+  int split;             // pairs of CTAs that share a tile
 };
 
 struct PlaneControl {
@@ -82,12 +105,66 @@ struct PlaneControl {
 };
 static_assert(sizeof(PlaneControl) <= 1024, "control block");
 
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// All threads of the cluster; what was written before is seen behind it.
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same place in another CTA's shared memory.
+__device__ __forceinline__ unsigned cluster_addr(unsigned addr, unsigned rank) {
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive(unsigned bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];"
+               ::"r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void cluster_store(unsigned addr, float a, float b, float c,
+                                              float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a),
+               "f"(b), "f"(c), "f"(d)
+               : "memory");
+}
+
+// D = f32, A = B = f16, M = N = 256 by two CTAs.
+__device__ __forceinline__ unsigned pair_desc(bool a_mn, bool b_mn) {
+  return (1u << 4) | ((unsigned)a_mn << 15) | ((unsigned)b_mn << 16) |
+         ((unsigned)(PL_TILE >> 3) << 17) | ((unsigned)(PL_TILE >> 4) << 24);
+}
+__device__ __forceinline__ void pair_mma(unsigned tmem_d, unsigned long long da,
+                                         unsigned long long db, unsigned idesc,
+                                         unsigned accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives at the barrier in both CTAs of the pair (`mask`) once the MMAs are done.
+__device__ __forceinline__ void pair_commit(unsigned long long* bar,
+                                            unsigned short mask) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster."
+      "multicast::cluster.b64 [%0], %1;"
+      ::"r"(smem_u32(bar)), "h"(mask)
+      : "memory");
+}
+
 __device__ __forceinline__ void pl_load(unsigned dst, const CUtensorMap* map, int x,
-                                        int y, int z, unsigned long long* bar) {
+                                        int y, int z, unsigned bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::"
-      "complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      "complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
 
@@ -95,30 +172,13 @@ __device__ __forceinline__ void pl_load(unsigned dst, const CUtensorMap* map, in
 // box of 128 rows x 64 k; rows along the planes: two boxes of 64 k x 64 rows.
 __device__ __forceinline__ void pl_load_term(unsigned dst, const CUtensorMap* map,
                                              int mn, int r0, int kb, int term,
-                                             unsigned long long* bar) {
+                                             unsigned bar) {
   if (!mn) {
     pl_load(dst, map, kb * PL_BK, r0, term, bar);
   } else {
     pl_load(dst, map, r0, kb * PL_BK, term, bar);
     pl_load(dst + PL_TERM / 2, map, r0 + 64, kb * PL_BK, term, bar);
   }
-}
-
-// 32 columns of this lane's accumulator row.
-__device__ __forceinline__ void pl_ld32(unsigned taddr, unsigned (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, "
-      "%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
-        "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-        "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
 }
 
 // Two values as fp16 terms, rounded to nearest.  Beyond the range hi is infinite and
@@ -132,66 +192,100 @@ __device__ __forceinline__ void pl_split2(float y0, float y1, unsigned& hi,
   lo = *reinterpret_cast<const unsigned*>(&l);
 }
 
-// What an epilogue's warp has: 64 columns c0.. of 32 rows r0.. (row: the lane), and
-// 4 KB of shared memory of its own.
+// What an epilogue gets at a time: 32 rows from r0 and 32 columns from c0, and 4 KB of
+// shared memory of the warp's own.  v[16 f + 4 j + 2 h + e] is row 16 f + 8 h +
+// lane / 4, column 8 j + 2 (lane % 4) + e: what the matrix stores and loads of shared
+// memory have in a register.
 struct PlaneTile {
   int r0, c0, lane;
   unsigned char* piece;
 };
 
-// v as planes, rows r0 + lane, and with `mirror` (a tile below the diagonal of a
-// symmetric result) its transpose.  Rows go out as 128 (transposed: 64) bytes, turned
-// in shared memory.
+__device__ __forceinline__ void st_matrix(unsigned addr, unsigned a, unsigned b,
+                                          unsigned c, unsigned d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};"
+               ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ void st_matrix_t(unsigned addr, unsigned a, unsigned b,
+                                            unsigned c, unsigned d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+               ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ void ld_matrix(unsigned addr, unsigned& a, unsigned& b,
+                                          unsigned& c, unsigned& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+               : "r"(addr)
+               : "memory");
+}
+
+// 32 rows of 64 bytes in shared memory, without bank conflicts: 16-byte word j of a row.
+__device__ __forceinline__ int row64_off(int row, int j) {
+  return row * 64 + ((j ^ ((row >> 1) & 3)) << 4);
+}
+
+// A tile's 16-bit pairs (w[8 f + 2 j + h], one word per row and column pair) from the
+// registers to rows of 64 bytes, or transposed.
+__device__ __forceinline__ void pl_put_pairs(unsigned piece, const unsigned (&w)[16],
+                                             int lane) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    st_matrix(piece + row64_off(lane, j), w[2 * j], w[2 * j + 1], w[8 + 2 * j],
+              w[8 + 2 * j + 1]);
+}
+__device__ __forceinline__ void pl_put_pairs_t(unsigned piece, const unsigned (&w)[16],
+                                               int lane) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {            // eight rows: 16-byte word g of a column
+    const int at = 8 * (g >> 1) + (g & 1);
+    st_matrix_t(piece + row64_off(lane, g), w[at], w[at + 2], w[at + 4], w[at + 6]);
+  }
+}
+
+// Those rows to memory, 16 bytes a lane: row r0 + r of `rows`, columns from c0 of
+// `cols` (a row's last word may pass its end: the plane has the room).
+__device__ __forceinline__ void pl_rows_out(unsigned piece, __half* base, int ld,
+                                            int r0, int rows, int c0, int cols,
+                                            int lane) {
+  const int j = lane & 3, r = lane >> 2;
+  __half* to = base + (long long)(r0 + r) * ld + c0 + 8 * j;
+  const unsigned from = piece + row64_off(r, j);   // (eight rows on: the same turn)
+  const int left = c0 + 8 * j < cols ? rows - r0 - r : 0;
+  const long long step = 8LL * ld;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "r"(from + 512 * i)
+                 : "memory");
+    if (8 * i < left) *reinterpret_cast<uint4*>(to) = x;
+    to += step;
+  }
+}
+
+// v as planes, and with `mirror` (below the diagonal of a symmetric result) its
+// transpose.
 __device__ __forceinline__ void pl_store_planes(const PlaneTile& t, const Planes& o,
-                                                const float (&v)[64], int M, int N,
+                                                const float (&v)[32], int M, int N,
                                                 int terms, bool mirror) {
-  unsigned char* const piece = t.piece;
-  const int lane = t.lane;
+  const unsigned piece = smem_u32(t.piece);
+  unsigned hi[16], lo[16];
 #pragma unroll
-  for (int term = 0; term < 2; ++term) {
-    if (term >= terms) break;
+  for (int i = 0; i < 16; ++i) pl_split2(v[2 * i], v[2 * i + 1], hi[i], lo[i]);
+#pragma unroll 1
+  for (int term = 0; term < terms; ++term) {
     __half* const base = o.p + (term ? o.plane : 0);
-    unsigned w[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      unsigned hi, lo;
-      pl_split2(v[2 * i], v[2 * i + 1], hi, lo);
-      w[i] = term ? lo : hi;
-    }
     __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      *reinterpret_cast<uint4*>(piece + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-          make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    pl_put_pairs(piece, hi, t.lane);
+    if (mirror) pl_put_pairs_t(piece + 2048, hi, t.lane);
     __syncwarp();
+    pl_rows_out(piece, base, o.ld, t.r0, M, t.c0, N, t.lane);
+    if (mirror) pl_rows_out(piece + 2048, base, o.ld, t.c0, N, t.r0, M, t.lane);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + (lane >> 3), j = lane & 7;
-      const uint4 x =
-          *reinterpret_cast<const uint4*>(piece + r * 128 + ((j ^ (r & 7)) << 4));
-      // (a row's last words may pass its end: the plane has the room)
-      if (t.r0 + r < M && t.c0 + 8 * j < N)
-        *reinterpret_cast<uint4*>(base + (long long)(t.r0 + r) * o.ld + t.c0 +
-                                  8 * j) = x;
-    }
-    if (!mirror) continue;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      __half* const at = reinterpret_cast<__half*>(piece) + 64 * i + lane;
-      const __half2 x = *reinterpret_cast<const __half2*>(&w[i]);
-      at[0] = __low2half(x);
-      at[32] = __high2half(x);
-    }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = 8 * i + (lane >> 2), j = lane & 3;
-      const uint4 x = *reinterpret_cast<const uint4*>(piece + c * 64 + 16 * j);
-      if (t.c0 + c < N && t.r0 + 8 * j < M)
-        *reinterpret_cast<uint4*>(base + (long long)(t.c0 + c) * o.ld + t.r0 +
-                                  8 * j) = x;
-    }
+    for (int i = 0; i < 16; ++i) hi[i] = lo[i];
   }
 }
 
@@ -201,11 +295,11 @@ __device__ __forceinline__ const PlaneProblem& pl_problem(const PlaneLaunch<N>& 
                                                           int tile) {
   int f = 0;
   for (int i = 1; i < l.n; ++i)
-    if (l.p[i].tile_begin <= tile) f = i;
+    if (l.p[i].f.tile_begin <= tile) f = i;
   return l.p[f];
 }
 
-__device__ __forceinline__ void pl_tile_at(const PlaneProblem& g, int tile, int& m0,
+__device__ __forceinline__ void pl_tile_at(const PlaneFields& g, int tile, int& m0,
                                            int& n0) {
   const int t = tile - g.tile_begin;
   int bi, bj;
@@ -215,12 +309,12 @@ __device__ __forceinline__ void pl_tile_at(const PlaneProblem& g, int tile, int&
     bi = t / g.tiles_n;
     bj = t - bi * g.tiles_n;
   }
-  m0 = bi * PL_BM;
-  n0 = bj * PL_BM;
+  m0 = bi * PL_TILE;
+  n0 = bj * PL_TILE;
 }
 
-// Epi: the epilogue's type; epi.store(problem, tile, v) takes the sums of a warp's
-// part of a tile, unscaled.
+// Epi: the epilogue's type; epi.store(problem, tile, v, mirror) takes the sums of a
+// PlaneTile, unscaled.
 template <int N, typename Epi>
 __global__ void __launch_bounds__(PL_THREADS, 1)
 plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
@@ -235,7 +329,11 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int stage_bytes = l.terms * PL_TERM;
   const int stages = PL_STAGE_BYTES / stage_bytes;
-  const bool cross = l.terms > 2, cut = l.terms == 4;
+  const bool cut = l.terms == 4;
+  const int S = l.split;
+  const unsigned rank = cluster_rank(), first = rank & ~1u, side = rank & 1u;
+  const int part = (int)(rank >> 1);               // of a shared sum
+  const int tile0 = blockIdx.x / (2 * S), step = gridDim.x / (2 * S);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -245,7 +343,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
       }
       for (int b = 0; b < 2; ++b) {
         mbar_init(&ctl->accum[b], 1);
-        mbar_init(&ctl->drained[b], PL_EPI_WARPS);
+        mbar_init(&ctl->drained[b], 2 * PL_EPI_WARPS);
       }
       ctl->abort_flag = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -253,33 +351,48 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
     __syncwarp();
   } else if (warp == 1) {
     asm volatile(
-        "tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+        "tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
         ::"r"(smem_u32(&ctl->tmem_base)), "r"(PL_COLS)
         : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;"
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;"
                  ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  cluster_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   let_next_launch_begin();
-  wait_for_launch_before();
+  // (each role waits for the launch before where it first reads or writes memory)
 
   const unsigned tmem = ctl->tmem_base;
+  // k-blocks of a tile that this pair adds up
+  auto range = [&](const PlaneFields& g, int& kb0, int& nkb) {
+    const int all = (g.K + PL_BK - 1) / PL_BK, each = (all + S - 1) / S;
+    kb0 = min(part * each, all);
+    nkb = min(each, all - kb0);
+  };
   if (warp == 0) {
     if (elect_one()) {
-      // what the launch before wrote is read by the copy engine
-      asm volatile("fence.proxy.async;" ::: "memory");
       int it = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < l.tiles; tile += gridDim.x) {
-        const PlaneProblem& g = pl_problem(l, tile);
-        int m0, n0;
+      for (int tile = tile0; ok && tile < l.tiles; tile += step) {
+        const PlaneProblem& p = pl_problem(l, tile);
+        const PlaneFields g = p.f;
+        int m0, n0, kb0, nkb;
         pl_tile_at(g, tile, m0, n0);
+        range(g, kb0, nkb);
         const bool share = g.same && m0 == n0;
-        const int nkb = (g.K + PL_BK - 1) / PL_BK, ta = g.ta, tb = g.tb;
+        const int ta = g.ta, tb = g.tb;
         const unsigned bytes = (share ? ta : ta + tb) * PL_TERM;
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
+        const int ra = m0 + PL_ROWS * side, rb = n0 + PL_ROWS * side;
+        if (it == 0) {
+          asm volatile("prefetch.tensormap [%0];" ::"l"(&p.ma) : "memory");
+          asm volatile("prefetch.tensormap [%0];" ::"l"(&p.mb) : "memory");
+          wait_for_launch_before();
+          // what it wrote is read by the copy engine
+          asm volatile("fence.proxy.async;" ::: "memory");
+        }
+        for (int kb = kb0; kb < kb0 + nkb; ++kb, ++it) {
           const int s = it % stages;
           if (it >= stages &&
               !mbar_wait_status(&ctl->empty[s], ((it / stages) - 1) & 1,
@@ -287,42 +400,47 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
             ok = false;
             break;
           }
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-                       ::"r"(smem_u32(&ctl->full[s])), "r"(bytes)
-                       : "memory");
+          // both CTAs' loads count at the first one's barrier
+          const unsigned bar = cluster_addr(smem_u32(&ctl->full[s]), first);
+          if (side == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
+                         ::"r"(smem_u32(&ctl->full[s])), "r"(2 * bytes)
+                         : "memory");
           const unsigned st = smem_u32(smem + s * stage_bytes);
           for (int t = 0; t < ta; ++t)
-            pl_load_term(st + t * PL_TERM, &g.ma, g.a_mn, m0, kb, t, &ctl->full[s]);
+            pl_load_term(st + t * PL_TERM, &p.ma, g.a_mn, ra, kb, t, bar);
           if (share) continue;
           for (int t = 0; t < tb; ++t)
-            pl_load_term(st + (ta + t) * PL_TERM, &g.mb, g.b_mn, n0, kb, t,
-                         &ctl->full[s]);
+            pl_load_term(st + (ta + t) * PL_TERM, &p.mb, g.b_mn, rb, kb, t, bar);
         }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (elect_one()) {
+    if (side == 0 && elect_one()) {
+      const unsigned short both = (unsigned short)(3u << first);
       int it = 0, seg = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < l.tiles; tile += gridDim.x) {
-        const PlaneProblem& g = pl_problem(l, tile);
-        int m0, n0;
+      for (int tile = tile0; ok && tile < l.tiles; tile += step) {
+        const PlaneFields g = pl_problem(l, tile).f;
+        int m0, n0, kb0, nkb;
         pl_tile_at(g, tile, m0, n0);
+        range(g, kb0, nkb);
         const bool share = g.same && m0 == n0;
-        const int nkb = (g.K + PL_BK - 1) / PL_BK, ta = g.ta, tb = g.tb;
+        const int ta = g.ta, tb = g.tb;
         const bool amn = g.a_mn, bmn = g.b_mn;
-        const unsigned idesc = tc_half_desc(PL_BM, amn, bmn);
+        const unsigned idesc = pair_desc(amn, bmn);
         // from 16 k to the next (16-byte units)
         const unsigned long long adv_a = (amn ? 2048 : 32) >> 4;
         const unsigned long long adv_b = (bmn ? 2048 : 32) >> 4;
+        const unsigned long long lo = PL_TERM >> 4;
         unsigned d = 0;
         for (int kb = 0; kb < nkb; ++kb, ++it) {
           const int s = it % stages;
           const bool fresh = kb == 0 || (cut && kb % PL_SEGMENT == 0);
           if (fresh) {
             const int b = seg & 1;
-            d = tmem + b * (PL_COLS / 2);
+            d = tmem + b * PL_TILE;
             if (seg >= 2 &&
                 !mbar_wait_status(&ctl->drained[b], ((seg >> 1) - 1) & 1,
                                   &ctl->abort_flag, status)) {
@@ -338,45 +456,58 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const unsigned sa = smem_u32(smem + s * stage_bytes);
           const unsigned sb = share ? sa : sa + ta * PL_TERM;
-          unsigned long long a =
+          const unsigned long long a =
               amn ? tc_smem_desc_mn(sa, PL_TERM / 2) : tc_smem_desc(sa);
-          unsigned long long b =
+          const unsigned long long b =
               bmn ? tc_smem_desc_mn(sb, PL_TERM / 2) : tc_smem_desc(sb);
-          const unsigned long long lo = PL_TERM >> 4;
+          unsigned acc = !fresh;
+          if (tb == 2) {
 #pragma unroll
-          for (int kk = 0; kk < PL_BK / 16; ++kk, a += adv_a, b += adv_b) {
-            const unsigned acc = !fresh || kk != 0;
-            if (tb == 2) tc_mma_half(d + PL_BM, a, b + lo, idesc, acc);
-            if (ta == 2) tc_mma_half(d + PL_BM, a + lo, b, idesc, acc | (tb == 2));
-            tc_mma_half(d, a, b, idesc, acc);
+            for (int kk = 0; kk < PL_BK / 16; ++kk) {
+              pair_mma(d, a + kk * adv_a, b + lo + kk * adv_b, idesc, acc);
+              acc = 1;
+            }
           }
-          tc_commit(&ctl->empty[s]);
+          if (ta == 2) {
+#pragma unroll
+            for (int kk = 0; kk < PL_BK / 16; ++kk) {
+              pair_mma(d, a + lo + kk * adv_a, b + kk * adv_b, idesc, acc);
+              acc = 1;
+            }
+          }
+#pragma unroll
+          for (int kk = 0; kk < PL_BK / 16; ++kk) {
+            pair_mma(d, a + kk * adv_a, b + kk * adv_b, idesc, acc);
+            acc = 1;
+          }
+          pair_commit(&ctl->empty[s], both);
           if (kb + 1 == nkb || (cut && (kb + 1) % PL_SEGMENT == 0)) {
-            tc_commit(&ctl->accum[seg & 1]);
+            pair_commit(&ctl->accum[seg & 1], both);
             ++seg;
           }
         }
       }
     }
     __syncwarp();
-  } else {
-    const int q = warp & 3, h = (warp - 2) >> 2;
+  } else if (warp >= 4) {
+    const int q = warp & 3, h = (warp >> 2) - 1;
     PlaneTile t;
     t.lane = lane;
-    t.piece = pieces + (warp - 2) * PL_PIECE;
+    t.piece = pieces + (warp - 4) * PL_PIECE;
     int seg = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < l.tiles; tile += gridDim.x) {
-      const PlaneProblem& g = pl_problem(l, tile);
-      int m0, n0;
+    wait_for_launch_before();
+    for (int tile = tile0; ok && tile < l.tiles; tile += step) {
+      const PlaneFields g = pl_problem(l, tile).f;
+      int m0, n0, kb0, nkb;
       pl_tile_at(g, tile, m0, n0);
-      t.r0 = m0 + 32 * q;
-      t.c0 = n0 + 64 * h;
-      const int nkb = (g.K + PL_BK - 1) / PL_BK;
-      const int nseg = cut ? (nkb + PL_SEGMENT - 1) / PL_SEGMENT : 1;
-      float v[64];
+      range(g, kb0, nkb);
+      t.r0 = m0 + PL_ROWS * side + 32 * q;
+      const bool mirror = g.lower && m0 != n0;
+      const int nseg = cut ? (nkb + PL_SEGMENT - 1) / PL_SEGMENT : (nkb > 0 ? 1 : 0);
+      float v[128];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) v[i] = 0.f;
+      for (int i = 0; i < 128; ++i) v[i] = 0.f;
 #pragma unroll 1
       for (int k = 0; k < nseg; ++k, ++seg) {
         const int b = seg & 1;
@@ -385,33 +516,98 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const unsigned at = tmem + ((unsigned)(32 * q) << 16) + b * (PL_COLS / 2) +
-                            64 * h;
+        const unsigned at = tmem + ((unsigned)(32 * q) << 16) + b * PL_TILE + 128 * h;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          unsigned x[32], y[32];
-          pl_ld32(at + 32 * half, x);
-          if (cross) pl_ld32(at + PL_BM + 32 * half, y);
+        for (int u = 0; u < 4; ++u) {
+          float x[16], y[16];
+          tc_ld_16x32(at + 32 * u, x);
+          tc_ld_16x32(at + (16u << 16) + 32 * u, y);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float sum = __uint_as_float(x[i]);
-            if (cross) sum += __uint_as_float(y[i]);
-            v[32 * half + i] += sum;
+          for (int i = 0; i < 16; ++i) {
+            v[32 * u + i] += x[i];
+            v[32 * u + 16 + i] += y[i];
           }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->drained[b]);
+        if (lane == 0)
+          cluster_arrive(cluster_addr(smem_u32(&ctl->drained[b]), first));
+      }
+      if (S > 1) {
+        // A shared sum (the cluster's only tile): the pairs own a part of the columns
+        // each, a multiple of the 32 that 32 registers hold.  Parts lie by pair, rows'
+        // quarter, four registers, lane.
+        const int width = PL_TILE / S, groups = width / 4;
+        const unsigned base = smem_u32(smem);
+        cluster_sync();                      // the MMAs have read all stages
+        if (ok) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int col = 128 * h + 4 * i, owner = col / width;
+            const unsigned to = cluster_addr(base, 2 * owner + side);
+            cluster_store(to + ((part * 4 + q) * groups + (col - owner * width) / 4) *
+                                   512 + lane * 16,
+                          v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+        }
+        cluster_sync();
+        if (!ok) break;
+        // (of 32 columns in all the second half of the warps has none)
+        const int mine = max(32, width / 2);
+#pragma unroll 1
+        for (int c0 = h * mine; c0 < min((h + 1) * mine, width); c0 += 32) {
+          float x[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = 0.f;
+#pragma unroll 1
+          for (int p = 0; p < S; ++p) {
+            const unsigned char* from =
+                smem + ((p * 4 + q) * groups + c0 / 4) * 512 + lane * 16;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 w = *reinterpret_cast<const float4*>(from + 512 * i);
+              x[4 * i] += w.x;
+              x[4 * i + 1] += w.y;
+              x[4 * i + 2] += w.z;
+              x[4 * i + 3] += w.w;
+            }
+          }
+          t.c0 = n0 + part * width + c0;
+          if (t.r0 < g.M && t.c0 < g.N) epi.store(g, t, x, mirror);
+        }
+        break;
       }
       if (!ok) break;
-      if (t.r0 < g.M && t.c0 < g.N)
-        epi.store(g, t, v, g.lower && m0 != n0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        t.c0 = n0 + 128 * h + 32 * u;
+        float x[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = v[32 * u + i];
+        if (t.r0 < g.M && t.c0 < g.N) epi.store(g, t, x, mirror);
+      }
     }
+  }
+  if (S > 1 && warp < 4) {
+    cluster_sync();
+    cluster_sync();
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (warp == 1) tc_release(tmem, PL_COLS, ctl->abort_flag != 0);
+  // (nobody leaves while the other may still arrive at its barriers)
+  cluster_sync();
+  if (warp == 1) {
+    if (ctl->abort_flag != 0) {
+      // what is under way gets time to end (bounded: 64 us)
+#pragma unroll 1
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
+      __syncwarp();
+    }
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;"
+                 ::"r"(tmem), "r"(PL_COLS)
+                 : "memory");
+  }
 }
 
 // ----------------------------------------------------------------- host side
@@ -458,42 +654,123 @@ inline int plane_map(CUtensorMap* map, const Planes& o, int rows, int cols, bool
   return KFAC_OK;
 }
 
+// What truncation takes from a segment's sum on average, made good.  An addition
+// loses half a unit in the last place of the sum so far, 2^-24 / m of it with a
+// mantissa m that is log-uniform: 0.72 2^-24.  Of a sum that grows evenly (a diagonal;
+// on average over the places where its large term may stand, any other) the blocks'
+// cross terms, 8 additions, meet 0, 1 / n, 2 / n .. of the segment's n blocks' sum, and
+// the 4 n others 1 / 4n, 2 / 4n .. 1: 6 n - 3.5 whole ones.  Errors of orthogonalised
+// 4096 x 4096 and 1024 x 4096 against fp64, with and without:
+// 1.9e-6 and 3.0e-6, 2.3e-6 and 4.0e-6 (fp32 products: 4.3e-6, 3.7e-6).
+inline float plane_gain(int terms, int K) {
+  if (terms < 4) return 1.f;
+  const int n = std::min((K + PL_BK - 1) / PL_BK, PL_SEGMENT);
+  return 1.f + (6 * n - 3.5f) * 0.72f * exp2f(-24);
+}
+
 // Numbers the tiles of l.p[0 .. l.n).
 template <int N>
 void plane_number_tiles(PlaneLaunch<N>& l) {
   int total = 0;
   for (int i = 0; i < l.n; ++i) {
-    PlaneProblem& g = l.p[i];
-    const int tm = (g.M + PL_BM - 1) / PL_BM, tn = (g.N + PL_BM - 1) / PL_BM;
+    PlaneFields& g = l.p[i].f;
+    const int tm = (g.M + PL_TILE - 1) / PL_TILE, tn = (g.N + PL_TILE - 1) / PL_TILE;
     g.tiles_n = tn;
     g.tile_begin = total;
     total += g.lower ? tm * (tm + 1) / 2 : tm * tn;
+    g.gain = plane_gain(g.ta + g.tb, g.K);
   }
   l.tiles = total;
-  l.terms = l.n > 0 ? l.p[0].ta + l.p[0].tb : 0;
+  l.terms = l.n > 0 ? l.p[0].f.ta + l.p[0].f.tb : 0;
+  l.split = 1;
+}
+
+// How many pairs share a tile: as many as a count of cycles comes out least for, with
+// `room[i]` clusters of 2^i pairs on the GPU at a time.  A k-block takes an MMA of 128
+// cycles for each 16 k and product of terms; a tile's start and end 6000 (beside the
+// next one's MMAs 2000), 18000 with a shared sum: the parts go through distributed
+// shared memory at 20 bytes a cycle and SM.  512 x 4608, whose X X^T has three tiles of
+// 72 k-blocks: five steps 342 us with eight pairs a tile, 373 with four; 2048 x 2048,
+// whose 36 tiles of 32 k-blocks do not all find room in pairs of pairs (33 do): 700 us
+// with one, 788 with two.
+template <int N>
+int plane_split(const PlaneLaunch<N>& l, const int* room) {
+  const double cycles = (l.terms - 1) * 4 * 132.0;
+  double best = 0;
+  int split = 1;
+  for (int i = 0, s = 1; s <= PL_SPLIT_MAX; ++i, s *= 2) {
+    if (room[i] <= 0) break;
+    double longest = 0, sum = 0;
+    for (int k = 0; k < l.n; ++k) {
+      const int end = k + 1 < l.n ? l.p[k + 1].f.tile_begin : l.tiles;
+      const int kb = (l.p[k].f.K + PL_BK - 1) / PL_BK;
+      const double one = (kb + s - 1) / s * cycles + (s > 1 ? 18000 : 2000);
+      longest = std::max(longest, one);
+      sum += one * (end - l.p[k].f.tile_begin);
+    }
+    // (tiles of one size run in whole waves, of different sizes closer together)
+    const double waves = (double)l.tiles / room[i];
+    const double time =
+        std::max(longest, l.n == 1 ? sum / l.tiles * std::ceil(waves)
+                                   : sum / l.tiles * waves + longest / 2) +
+        (s > 1 ? 0 : 4000);
+    if (s == 1 || time < best) {
+      best = time;
+      split = s;
+    }
+  }
+  return split;
 }
 
 template <int N, typename Epi>
-int plane_launch(const char* name, const PlaneLaunch<N>& l, const Epi& epi,
-                 bool early, cudaStream_t stream) {
+int plane_launch(const char* name, PlaneLaunch<N>& l, const Epi& epi, bool early,
+                 cudaStream_t stream) {
   if (l.tiles == 0) return KFAC_OK;
   static std::mutex mu;
-  static bool done[64] = {false};
+  static int room[64][4];                      // 0: not asked yet
   int dev = 0;
   KFAC_CUDA(cudaGetDevice(&dev));
   KFAC_REQUIRE(dev >= 0 && dev < 64, "device index %d unsupported", dev);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(PL_THREADS);
+  cfg.dynamicSmemBytes = PL_SMEM;
+  cfg.stream = stream;
+  cfg.attrs = attr;
   {
     std::lock_guard<std::mutex> lock(mu);
-    if (!done[dev]) {
+    if (room[dev][0] == 0) {
       KFAC_CUDA(cudaFuncSetAttribute(plane_kernel<N, Epi>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      PL_SMEM));
-      done[dev] = true;
+      KFAC_CUDA(cudaFuncSetAttribute(plane_kernel<N, Epi>,
+                                     cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+      for (int i = 3; i >= 0; --i) {
+        attr[0].val.clusterDim.x = 2 << i;
+        cfg.gridDim = dim3((2 << i) * 64);
+        cfg.numAttrs = 1;
+        int n = 0;
+        KFAC_CUDA(cudaOccupancyMaxActiveClusters(&n, plane_kernel<N, Epi>, &cfg));
+        room[dev][i] = n > 0 ? n : -1;
+      }
+      KFAC_REQUIRE(room[dev][0] > 0, "%s: no room for a pair of blocks", name);
     }
   }
-  return launch_behind(name, early, plane_kernel<N, Epi>,
-                       std::min(l.tiles, sm_count()), PL_THREADS, PL_SMEM, stream, l,
-                       epi);
+  l.split = plane_split(l, room[dev]);
+  const int cluster = 2 * l.split;
+  const int clusters = l.split > 1 ? l.tiles : std::min(l.tiles, room[dev][0]);
+  attr[0].val.clusterDim.x = cluster;
+  cfg.gridDim = dim3(cluster * clusters);
+  cfg.numAttrs = early ? 2 : 1;
+  KFAC_CUDA(cudaLaunchKernelEx(&cfg, plane_kernel<N, Epi>, l, epi));
+  KFAC_LAUNCH_CHECK(name);
+  return KFAC_OK;
 }
 
 }  // namespace kfac

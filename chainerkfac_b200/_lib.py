@@ -125,6 +125,9 @@ SIGNATURES = {
     'kfac_orthogonalize': (I, [I, I, c_int_p, c_int_p, c_void_pp, c_void_pp,
                                c_void_pp, c_float_p, I, c_float_p, F, F, F,
                                VP, SZ, VP]),
+    'kfac_precondition_embedding_workspace_bytes': (SZ, [I64, I]),
+    'kfac_precondition_embedding': (I, [I64, I] + [VP] * 7 +
+                                    [F, F, VP, SZ, VP]),
     'kfac_token_counts_workspace_bytes': (SZ, [I64]),
     'kfac_token_counts': (I, [VP, I, I64, I64, I, I64, F, F, VP, VP, VP, SZ,
                               VP]),

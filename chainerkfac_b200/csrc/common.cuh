@@ -61,6 +61,9 @@ int diag_status_read(int* out);
 // Status word of the orthogonalisation's products (ortho.cu).
 int ortho_status_read(int* out);
 
+// And of an embedding's (embed_precond.cu).
+int embed_status_read(int* out);
+
 // Number of streaming multiprocessors of the current device (cached).
 int sm_count();
 

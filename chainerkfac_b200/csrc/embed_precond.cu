@@ -1,0 +1,358 @@
+// The K-FAC step of a token embedding (vocab x width), a fully connected layer on rows
+// with a single one: its input factor is a diagonal, so
+//
+//   kf = diag(1 / (A + delta)) grad G_inv,  v = momentum v - lr kf,  W = W + v.
+//
+// A batch reaches few of the tokens.  The first launch reads the gradient once, a row a
+// warp: a row of zeros has its update at once (kf = 0), any other goes as two fp16
+// terms, scaled by its own power of two, into the next free row of the planes
+// (planes.cuh) that are multiplied by G_inv; which row of the planes makes no
+// difference to its values.  The second launch multiplies as many rows as there are,
+// and its epilogue scales, scatters and updates them.
+//
+// Bound: HBM, 24 bytes an element (gradient in, kf out, velocity and weight in and
+// out), where the batch reaches few tokens; else the products, three MMAs each.
+#include <algorithm>
+
+#include "planes.cuh"
+
+namespace kfac {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kTopExp = 14;        // a row's largest value: 2^14 and more, below 2^15
+
+struct EmbedStep {
+  const float* G;                  // width x width, symmetric
+  const float* A;
+  const float* damping;            // one value
+  const float* grad;
+  float* kf;                       // or null
+  float* param;                    // or null, with mom
+  float* mom;
+  float lr, momentum;
+  int vocab, width;
+  Planes rows, g;
+  int* count;                      // rows of `rows`
+  int* index;                      // their tokens
+  int* row_exp;                    // of a row of `rows`
+  int* col_exp;                    // of a row (and column) of G
+  bool vec;                        // rows of 16-byte words
+};
+
+// Exponent of a row's largest value, by a warp; kNoExp: zeros.
+__device__ __forceinline__ int row_top(const float* x, int width, bool vec, int lane) {
+  int top = kNoExp;
+  if (vec) {
+    const float4* x4 = reinterpret_cast<const float4*>(x);
+    const int n = width >> 2;
+#pragma unroll 1
+    for (int k0 = lane; k0 < n; k0 += 256) {
+      float4 y[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) y[u] = x4[min(k0 + 32 * u, n - 1)];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        top = max(top, max(max(exp_of(y[u].x), exp_of(y[u].y)),
+                           max(exp_of(y[u].z), exp_of(y[u].w))));
+    }
+  } else {
+#pragma unroll 8
+    for (int k = lane; k < width; k += 32) top = max(top, exp_of(x[k]));
+  }
+  return __reduce_max_sync(0xffffffffu, top);
+}
+
+// x 2^s as planes, row `to`.
+__device__ __forceinline__ void pack_planes(const float* x, int width, bool vec,
+                                            const Planes& o, int to, int s, int lane) {
+  __half* const hi = o.p + (long long)to * o.ld;
+#pragma unroll 4
+  for (int k = 4 * lane; k < width; k += 128) {
+    float y[4];
+    if (vec) {
+      const float4 w = *reinterpret_cast<const float4*>(x + k);
+      y[0] = w.x; y[1] = w.y; y[2] = w.z; y[3] = w.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = k + e < width ? x[k + e] : 0.f;
+    }
+    uint2 h, l;
+    pl_split2(scale_exp(y[0], s), scale_exp(y[1], s), h.x, l.x);
+    pl_split2(scale_exp(y[2], s), scale_exp(y[3], s), h.y, l.y);
+    *reinterpret_cast<uint2*>(hi + k) = h;
+    *reinterpret_cast<uint2*>(hi + o.plane + k) = l;
+  }
+}
+
+// The update of a row without a gradient.
+__device__ __forceinline__ void rest_row(const EmbedStep& e, long long at, int lane) {
+  if (e.vec) {
+    const int n = e.width >> 2;
+#pragma unroll 1
+    for (int k0 = lane; k0 < n; k0 += 128) {
+      float4 v[4], p[4];
+      if (e.param != nullptr) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int k = min(k0 + 32 * u, n - 1);
+          v[u] = reinterpret_cast<const float4*>(e.mom + at)[k];
+          p[u] = reinterpret_cast<const float4*>(e.param + at)[k];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int k = k0 + 32 * u;
+        if (k >= n) break;
+        if (e.kf != nullptr)
+          reinterpret_cast<float4*>(e.kf + at)[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (e.param == nullptr) continue;
+        v[u].x *= e.momentum; v[u].y *= e.momentum;
+        v[u].z *= e.momentum; v[u].w *= e.momentum;
+        reinterpret_cast<float4*>(e.mom + at)[k] = v[u];
+        p[u].x += v[u].x; p[u].y += v[u].y; p[u].z += v[u].z; p[u].w += v[u].w;
+        reinterpret_cast<float4*>(e.param + at)[k] = p[u];
+      }
+    }
+    return;
+  }
+#pragma unroll 4
+  for (int k = lane; k < e.width; k += 32) {
+    if (e.kf != nullptr) e.kf[at + k] = 0.f;
+    if (e.param == nullptr) continue;
+    const float v = e.momentum * e.mom[at + k];
+    e.mom[at + k] = v;
+    e.param[at + k] += v;
+  }
+}
+
+__global__ void __launch_bounds__(kThreads)
+embed_rows_kernel(const __grid_constant__ EmbedStep e) {
+  let_next_launch_begin();
+  const int lane = threadIdx.x & 31;
+  const long long step = (long long)gridDim.x * kWarps;
+  // the rows of G first, then the gradient's
+  for (long long i = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+       i < (long long)e.width + e.vocab; i += step) {
+    const bool of_g = i < e.width;
+    const long long row = of_g ? i : i - e.width;
+    const float* x = (of_g ? e.G : e.grad) + row * e.width;
+    const int top = row_top(x, e.width, e.vec, lane);
+    if (top == kNoExp && !of_g) {
+      rest_row(e, row * e.width, lane);
+      continue;
+    }
+    const int s = top == kNoExp ? 0 : kTopExp - top;
+    int to = (int)row;
+    if (!of_g) {
+      if (lane == 0) to = atomicAdd(e.count, 1);
+      to = __shfl_sync(0xffffffffu, to, 0);
+    }
+    pack_planes(x, e.width, e.vec, of_g ? e.g : e.rows, to, s, lane);
+    if (lane == 0) {
+      (of_g ? e.col_exp : e.row_exp)[to] = -s;
+      if (!of_g) e.index[to] = (int)row;
+    }
+  }
+}
+
+struct EpiEmbed {
+  EmbedStep e;
+
+  __device__ __forceinline__ void store(const PlaneFields& g, const PlaneTile& t,
+                                        float (&v)[32], bool) const {
+    const unsigned piece = smem_u32(t.piece);
+    const int lane = t.lane, width = e.width;
+    // of row `lane`
+    const int r = min(t.r0 + lane, g.M - 1);
+    const int token = e.index[r], re = e.row_exp[r];
+    const float inv = 1.f / (e.A[token] + *e.damping);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= g.gain;
+    __syncwarp();
+    pl_put_floats(piece, v, lane);
+    __syncwarp();
+    const int rows = min(32, g.M - t.r0);
+    const bool fused = e.param != nullptr;
+    if (e.vec) {
+      const int c = t.c0 + 4 * (lane & 7);
+      const bool live = c < width;
+      int ce[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ce[k] = live ? e.col_exp[c + k] : 0;
+#pragma unroll
+      for (int i0 = 0; i0 < 32; i0 += 8) {
+        float4 old_v[2], old_p[2];
+        long long at[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = i0 + 4 * u + (lane >> 3);
+          at[u] = (long long)__shfl_sync(0xffffffffu, token, row) * width + c;
+          if (fused && live && row < rows) {
+            old_v[u] = *reinterpret_cast<const float4*>(e.mom + at[u]);
+            old_p[u] = *reinterpret_cast<const float4*>(e.param + at[u]);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = i0 + 4 * u + (lane >> 3);
+          const int n = __shfl_sync(0xffffffffu, re, row);
+          const float f = __shfl_sync(0xffffffffu, inv, row);
+          if (!live || row >= rows) continue;
+          float4 x = pl_word(piece, row, lane & 7);
+          x.x = scale_exp(x.x, n + ce[0]) * f;
+          x.y = scale_exp(x.y, n + ce[1]) * f;
+          x.z = scale_exp(x.z, n + ce[2]) * f;
+          x.w = scale_exp(x.w, n + ce[3]) * f;
+          if (e.kf != nullptr) *reinterpret_cast<float4*>(e.kf + at[u]) = x;
+          if (!fused) continue;
+          float4 w = old_v[u];
+          w.x = e.momentum * w.x - e.lr * x.x;
+          w.y = e.momentum * w.y - e.lr * x.y;
+          w.z = e.momentum * w.z - e.lr * x.z;
+          w.w = e.momentum * w.w - e.lr * x.w;
+          *reinterpret_cast<float4*>(e.mom + at[u]) = w;
+          w.x += old_p[u].x;
+          w.y += old_p[u].y;
+          w.z += old_p[u].z;
+          w.w += old_p[u].w;
+          *reinterpret_cast<float4*>(e.param + at[u]) = w;
+        }
+      }
+      return;
+    }
+    const int c = t.c0 + lane;
+    const int ce = c < width ? e.col_exp[c] : 0;
+#pragma unroll 4
+    for (int row = 0; row < rows; ++row) {
+      const long long at = (long long)__shfl_sync(0xffffffffu, token, row) * width + c;
+      const int n = __shfl_sync(0xffffffffu, re, row);
+      const float f = __shfl_sync(0xffffffffu, inv, row);
+      if (c >= width) continue;
+      const float x = scale_exp(pl_float(piece, row, lane), n + ce) * f;
+      if (e.kf != nullptr) e.kf[at] = x;
+      if (!fused) continue;
+      const float w = e.momentum * e.mom[at] - e.lr * x;
+      e.mom[at] = w;
+      e.param[at] += w;
+    }
+  }
+};
+
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+Planes place(char* ws, size_t& at, long long rows, int cols) {
+  Planes p;
+  p.ld = (cols + 7) & ~7;
+  p.plane = rows * p.ld;
+  p.p = reinterpret_cast<__half*>(ws + at);
+  at += up256((size_t)p.plane * 4);
+  return p;
+}
+
+// Lays a call's scratch out behind `ws`; the bytes it takes.
+size_t lay_out(int64_t vocab, int width, char* ws, EmbedStep* e) {
+  size_t at = 0;
+  const Planes rows = place(ws, at, vocab, width), g = place(ws, at, width, width);
+  int* const ints = reinterpret_cast<int*>(ws + at);
+  const size_t v = up256((size_t)vocab * 4), w = up256((size_t)width * 4);
+  at += 256 + 2 * v + w;
+  if (e != nullptr) {
+    e->rows = rows;
+    e->g = g;
+    e->count = ints;
+    e->index = ints + 64;
+    e->row_exp = ints + 64 + v / 4;
+    e->col_exp = ints + 64 + 2 * (v / 4);
+  }
+  return at + 256;            // (the workspace may begin anywhere)
+}
+
+int check_shape(int64_t vocab, int width) {
+  KFAC_REQUIRE(vocab >= 1 && vocab < (1LL << 31) - 256 && width >= 1 &&
+                   width <= (1 << 20),
+               "precondition_embedding: a weight of %lld x %d", (long long)vocab, width);
+  // (tiles are numbered in 32 bits)
+  KFAC_REQUIRE(((vocab + 255) / 256) * (int64_t)((width + 255) / 256) < (1LL << 31),
+               "precondition_embedding: a weight of %lld x %d", (long long)vocab, width);
+  return KFAC_OK;
+}
+
+}  // namespace
+
+int embed_status_read(int* out) {
+  KFAC_CUDA(cudaMemcpyFromSymbol(out, g_plane_status, sizeof(int)));
+  return KFAC_OK;
+}
+
+}  // namespace kfac
+
+using namespace kfac;
+
+extern "C" size_t kfac_precondition_embedding_workspace_bytes(int64_t vocab,
+                                                              int width) {
+  return check_shape(vocab, width) == KFAC_OK ? lay_out(vocab, width, nullptr, nullptr)
+                                              : 0;
+}
+
+extern "C" int kfac_precondition_embedding(int64_t vocab, int width, const float* G_inv,
+                                           const float* A, const float* damping,
+                                           const float* grad, float* kf, float* param,
+                                           float* mom, float lr, float momentum,
+                                           void* workspace, size_t workspace_bytes,
+                                           void* stream) {
+  int rc = check_shape(vocab, width);
+  if (rc != KFAC_OK) return rc;
+  KFAC_REQUIRE(G_inv != nullptr && A != nullptr && damping != nullptr &&
+                   grad != nullptr,
+               "precondition_embedding: null pointer");
+  KFAC_REQUIRE((param == nullptr) == (mom == nullptr),
+               "precondition_embedding: a weight and its velocity go together");
+  KFAC_REQUIRE(kf != nullptr || param != nullptr,
+               "precondition_embedding: nowhere to go");
+  const size_t need = lay_out(vocab, width, nullptr, nullptr);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(KFAC_ERR_WORKSPACE,
+                "precondition_embedding: %zu bytes of workspace, %zu needed",
+                workspace == nullptr ? (size_t)0 : workspace_bytes, need);
+  char* ws = reinterpret_cast<char*>(
+      (reinterpret_cast<uintptr_t>(workspace) + 255) & ~(uintptr_t)255);
+  EmbedStep e = {};
+  e.G = G_inv;
+  e.A = A;
+  e.damping = damping;
+  e.grad = grad;
+  e.kf = kf;
+  e.param = param;
+  e.mom = mom;
+  e.lr = lr;
+  e.momentum = momentum;
+  e.vocab = (int)vocab;
+  e.width = width;
+  e.vec = (width & 3) == 0 &&
+          ((reinterpret_cast<uintptr_t>(G_inv) | reinterpret_cast<uintptr_t>(grad) |
+            reinterpret_cast<uintptr_t>(kf) | reinterpret_cast<uintptr_t>(param) |
+            reinterpret_cast<uintptr_t>(mom)) & 15) == 0;
+  lay_out(vocab, width, ws, &e);
+  cudaStream_t st = (cudaStream_t)stream;
+  KFAC_CUDA(cudaMemsetAsync(e.count, 0, sizeof(int), st));
+  const long long rows = vocab + width;
+  embed_rows_kernel<<<(unsigned)std::min<long long>((rows + kWarps - 1) / kWarps,
+                                                    (long long)sm_count() * 8),
+                      kThreads, 0, st>>>(e);
+  KFAC_LAUNCH_CHECK("embed_rows_kernel");
+  PlaneLaunch<1> l;
+  l.n = 1;
+  PlaneFields& g = l.p[0].f;
+  g = {};
+  g.M = (int)vocab;
+  g.N = g.K = width;
+  g.ta = g.tb = 2;
+  if ((rc = plane_map(&l.p[0].ma, e.rows, (int)vocab, width, false)) != KFAC_OK ||
+      (rc = plane_map(&l.p[0].mb, e.g, width, width, false)) != KFAC_OK)
+    return rc;
+  plane_number_tiles(l);
+  l.rows = e.count;
+  return plane_launch("embed products", l, EpiEmbed{e}, true, st);
+}

@@ -237,13 +237,6 @@ struct EpiPlanes {
 template <typename T>
 struct EpiLast {
   float alpha, keep, lr;
-
-  // 32 x 32 values as rows of 128 bytes in shared memory, 16-byte words turned by the
-  // row: what a lane reads back is a column, or a word, of a row.
-  static __device__ __forceinline__ unsigned at(unsigned piece, int row, int word) {
-    return piece + row * 128 + ((word ^ (row & 7)) << 4);
-  }
-
   __device__ __forceinline__ void store(const PlaneFields& g, const PlaneTile& t,
                                         float (&v)[32], bool) const {
     const unsigned piece = smem_u32(t.piece);
@@ -254,15 +247,7 @@ struct EpiLast {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] *= a;
     __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const int row = 16 * (i >> 4) + 8 * ((i >> 1) & 1) + (lane >> 2);
-      asm volatile("st.shared.v2.f32 [%0], {%1, %2};"
-                   ::"r"(at(piece, row, 2 * ((i >> 2) & 3) + ((lane & 3) >> 1)) +
-                         8 * (lane & 1)),
-                     "f"(v[i]), "f"(v[i + 1])
-                   : "memory");
-    }
+    pl_put_floats(piece, v, lane);
     __syncwarp();
     constexpr int W = 16 / sizeof(T);      // values of a 16-byte word
     const bool words =
@@ -277,14 +262,11 @@ struct EpiLast {
 #pragma unroll
       for (int i = 0; i < 32 / R; ++i) {
         if (r + R * i >= rows) break;
-        float x[W];
+        alignas(16) float x[W];
 #pragma unroll
         for (int k = 0; k < W / 4; ++k)
-          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(x[4 * k]), "=f"(x[4 * k + 1]), "=f"(x[4 * k + 2]),
-                         "=f"(x[4 * k + 3])
-                       : "r"(at(piece, r + R * i, W / 4 * (lane % L) + k))
-                       : "memory");
+          *reinterpret_cast<float4*>(&x[4 * k]) =
+              pl_word(piece, r + R * i, W / 4 * (lane % L) + k);
         Word o;
         if (dst != nullptr) {
 #pragma unroll
@@ -306,11 +288,7 @@ struct EpiLast {
     const long long first = (long long)t.r0 * N + c;
 #pragma unroll 4
     for (int i = 0; i < min(rows, 32); ++i) {
-      float x;
-      asm volatile("ld.shared.f32 %0, [%1];"
-                   : "=f"(x)
-                   : "r"(at(piece, i, lane >> 2) + 4 * (lane & 3))
-                   : "memory");
+      const float x = pl_float(piece, i, lane);
       const long long k = first + (long long)i * N;
       if (dst != nullptr) dst[k] = from_float<T>(x);
       if (param != nullptr)

@@ -93,6 +93,8 @@ struct PlaneLaunch {
   int tiles;
   int terms;             // of both operands
   int split;             // pairs of CTAs that share a tile
+  const int* rows;       // the rows of a launch's only problem, where the device counts
+                         // them (M is then the most there can be); or null
 };
 
 struct PlaneControl {
@@ -289,6 +291,40 @@ __device__ __forceinline__ void pl_store_planes(const PlaneTile& t, const Planes
   }
 }
 
+// 32 x 32 values as rows of 128 bytes in shared memory, 16-byte words turned by the row
+// (no bank conflicts): what a lane reads back is a column, or a word, of a row.
+__device__ __forceinline__ unsigned row128_at(unsigned piece, int row, int word) {
+  return piece + row * 128 + ((word ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ void pl_put_floats(unsigned piece, const float (&v)[32],
+                                              int lane) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    const int row = 16 * (i >> 4) + 8 * ((i >> 1) & 1) + (lane >> 2);
+    asm volatile("st.shared.v2.f32 [%0], {%1, %2};"
+                 ::"r"(row128_at(piece, row, 2 * ((i >> 2) & 3) + ((lane & 3) >> 1)) +
+                       8 * (lane & 1)),
+                   "f"(v[i]), "f"(v[i + 1])
+                 : "memory");
+  }
+}
+__device__ __forceinline__ float4 pl_word(unsigned piece, int row, int word) {
+  float4 x;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "r"(row128_at(piece, row, word))
+               : "memory");
+  return x;
+}
+__device__ __forceinline__ float pl_float(unsigned piece, int row, int col) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];"
+               : "=f"(x)
+               : "r"(row128_at(piece, row, col >> 2) + 4 * (col & 3))
+               : "memory");
+  return x;
+}
+
 // Which problem a tile belongs to.
 template <int N>
 __device__ __forceinline__ const PlaneProblem& pl_problem(const PlaneLaunch<N>& l,
@@ -371,11 +407,17 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
     kb0 = min(part * each, all);
     nkb = min(each, all - kb0);
   };
+  int tiles = l.tiles, counted = 0;
+  if (l.rows != nullptr) {
+    wait_for_launch_before();
+    counted = *reinterpret_cast<const volatile int*>(l.rows);
+    tiles = (counted + PL_TILE - 1) / PL_TILE * l.p[0].f.tiles_n;
+  }
   if (warp == 0) {
     if (elect_one()) {
       int it = 0;
       bool ok = true;
-      for (int tile = tile0; ok && tile < l.tiles; tile += step) {
+      for (int tile = tile0; ok && tile < tiles; tile += step) {
         const PlaneProblem& p = pl_problem(l, tile);
         const PlaneFields g = p.f;
         int m0, n0, kb0, nkb;
@@ -421,7 +463,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
       const unsigned short both = (unsigned short)(3u << first);
       int it = 0, seg = 0;
       bool ok = true;
-      for (int tile = tile0; ok && tile < l.tiles; tile += step) {
+      for (int tile = tile0; ok && tile < tiles; tile += step) {
         const PlaneFields g = pl_problem(l, tile).f;
         int m0, n0, kb0, nkb;
         pl_tile_at(g, tile, m0, n0);
@@ -497,8 +539,9 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
     int seg = 0;
     bool ok = true;
     wait_for_launch_before();
-    for (int tile = tile0; ok && tile < l.tiles; tile += step) {
-      const PlaneFields g = pl_problem(l, tile).f;
+    for (int tile = tile0; ok && tile < tiles; tile += step) {
+      PlaneFields g = pl_problem(l, tile).f;
+      if (l.rows != nullptr) g.M = counted;
       int m0, n0, kb0, nkb;
       pl_tile_at(g, tile, m0, n0);
       range(g, kb0, nkb);
@@ -683,6 +726,7 @@ void plane_number_tiles(PlaneLaunch<N>& l) {
   l.tiles = total;
   l.terms = l.n > 0 ? l.p[0].f.ta + l.p[0].f.tb : 0;
   l.split = 1;
+  l.rows = nullptr;
 }
 
 // How many pairs share a tile: as many as a count of cycles comes out least for, with
@@ -762,7 +806,8 @@ int plane_launch(const char* name, PlaneLaunch<N>& l, const Epi& epi, bool early
       KFAC_REQUIRE(room[dev][0] > 0, "%s: no room for a pair of blocks", name);
     }
   }
-  l.split = plane_split(l, room[dev]);
+  // (a cluster that shares a tile has one, so the number has to be known)
+  l.split = l.rows != nullptr ? 1 : plane_split(l, room[dev]);
   const int cluster = 2 * l.split;
   const int clusters = l.split > 1 ? l.tiles : std::min(l.tiles, room[dev][0]);
   attr[0].val.clusterDim.x = cluster;

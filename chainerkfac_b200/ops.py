@@ -964,6 +964,51 @@ def token_counts(ids, vocab, ignore_label=None, alpha=1.0, beta=0.0, out=None,
     return out
 
 
+def precondition_embedding(G_inv, A, damping, grad, kf=None, param=None,
+                           mom=None, lr=0.0, momentum=0.0):
+    """kf = diag(1 / (A + damping)) grad G_inv for the gradient of an
+    embedding's (vocab, width) weight, all float32: ``G_inv`` symmetric, ``A``
+    (vocab,), ``damping`` one element (a ``G_inv`` that lies column by column,
+    as ``torch.linalg`` leaves it, is the same matrix).  With the weight ``param`` and its
+    velocity ``mom``, mom = momentum * mom - lr * kf and param += mom as well.
+    Rows without a gradient get zeros in ``kf``, and cost no product."""
+    if G_inv.dim() == 2 and not G_inv.is_contiguous():
+        G_inv = G_inv.t()
+    for t, name in ((G_inv, 'G_inv'), (A, 'A'), (damping, 'damping'),
+                    (grad, 'grad'), (kf, 'kf'), (param, 'param'),
+                    (mom, 'mom')):
+        _chk(t, name)
+    if grad.dim() != 2:
+        raise ValueError('grad must have two dimensions')
+    if (param is None) != (mom is None):
+        raise ValueError('param and mom go together')
+    vocab, width = grad.shape
+    device = grad.device
+    _chk_shape(G_inv, (width, width), 'G_inv')
+    _chk_shape(A, (vocab,), 'A')
+    if damping.numel() != 1:
+        raise ValueError('damping must have one element')
+    for t, name in ((kf, 'kf'), (param, 'param'), (mom, 'mom')):
+        if t is not None:
+            _chk_shape(t, (vocab, width), name)
+    _chk_place(device, G_inv=G_inv, A=A, damping=damping, kf=kf, param=param,
+               mom=mom)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return precondition_embedding(G_inv, A, damping, grad, kf, param,
+                                          mom, lr, momentum)
+    if kf is None:
+        kf = torch.empty_like(grad)
+    lib = _lib.load()
+    ws = _scratch(lib.kfac_precondition_embedding_workspace_bytes(
+        vocab, width), device)
+    _lib.check(lib.kfac_precondition_embedding(
+        vocab, width, G_inv.data_ptr(), A.data_ptr(), damping.data_ptr(),
+        grad.data_ptr(), kf.data_ptr(), _p(param), _p(mom), lr, momentum,
+        ws.data_ptr(), ws.numel(), _stream()), 'kfac_precondition_embedding')
+    return kf
+
+
 # -- orthogonalised updates ---------------------------------------------------
 
 # a, b, c of X = a X + (b A + c A A) X: five steps take singular values between

@@ -566,6 +566,25 @@ int kfac_orthogonalize(int dtype, int count, const int* rows, const int* cols,
                        float decay, void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/* ------------------------------------------------- K-FAC step of an embedding
+ * An embedding's weight is (vocab x width); as a fully connected layer on rows
+ * with a single one its input factor is a diagonal A (kfac_token_counts) and
+ *     kf = diag(1 / (A + damping)) grad G_inv
+ * with G_inv (width x width) the damped inverse of its output factor, a
+ * symmetric matrix, and `damping` one device float (the value that the inverse
+ * plan added to the diagonal of A's place).  With a weight and its velocity,
+ *     mom = momentum * mom - lr * kf,   param = param + mom.
+ * kf or the pair may be NULL.  All fp32, dense, row-major.  Rows whose gradient
+ * is zero have kf = 0 and cost no product; one with values that are not finite
+ * gives NaN in its own row. */
+size_t kfac_precondition_embedding_workspace_bytes(int64_t vocab, int width);
+int kfac_precondition_embedding(int64_t vocab, int width, const float* G_inv,
+                                const float* A, const float* damping,
+                                const float* grad, float* kf, float* param,
+                                float* mom, float lr, float momentum,
+                                void* workspace, size_t workspace_bytes,
+                                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -132,3 +132,26 @@ def test_orthogonalize_refuses_what_is_not_a_matrix():
         with pytest.raises(ValueError):
             ops.orthogonalize([x], **bad)
     assert ops.orthogonalize([]) == []
+
+
+def test_precondition_embedding_calls_are_checked(lib):
+    step = lambda **k: lib.kfac_precondition_embedding(*({**dict(
+        vocab=100, width=12, G=FAKE, A=FAKE, damping=FAKE, grad=FAKE, kf=FAKE,
+        param=None, mom=None, lr=0.1, momentum=0.9, ws=FAKE, nbytes=1 << 30,
+        stream=None), **k}).values())
+    for bad in (dict(vocab=0), dict(width=0), dict(vocab=2 ** 31),
+                dict(width=2 ** 20 + 1), dict(G=None), dict(A=None),
+                dict(damping=None), dict(grad=None), dict(kf=None),
+                dict(param=FAKE), dict(mom=FAKE)):
+        assert step(**bad) == 1, bad
+        assert 'precondition_embedding' in message(lib)
+    assert step(ws=None) == 3 and step(nbytes=1000) == 3
+    need = lib.kfac_precondition_embedding_workspace_bytes
+    assert need(0, 5) == 0 and need(5, 0) == 0
+    for v, d in ((1, 1), (1000, 100), (32000, 1024)):
+        assert 4 * (v + d) * d <= need(v, d) <= \
+            4 * (v + d) * (d + 7) + 8 * v + 4 * d + 4096
+    from chainerkfac_b200 import _lib, ops
+    x = torch.zeros(3, 3)
+    with pytest.raises(_lib.KfacLibraryError, match='CUDA tensor'):
+        ops.precondition_embedding(x, x[0], x[0, :1], x)

@@ -14,3 +14,5 @@ from chainerkfac_b200.communicators import create_communicator  # NOQA
 from chainerkfac_b200.optimizers import fisher_blocks  # NOQA
 from chainerkfac_b200.optimizers.kfac import KFAC  # NOQA
 from chainerkfac_b200.optimizers.kfac import DistributedKFAC  # NOQA
+from chainerkfac_b200.optimizers.orthogonal import OrthogonalUpdateRule  # NOQA
+from chainerkfac_b200.embed_id import EmbedID  # NOQA

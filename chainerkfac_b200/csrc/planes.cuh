@@ -640,17 +640,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
   __syncthreads();
   // (nobody leaves while the other may still arrive at its barriers)
   cluster_sync();
-  if (warp == 1) {
-    if (ctl->abort_flag != 0) {
-      // what is under way gets time to end (bounded: 64 us)
-#pragma unroll 1
-      for (int i = 0; i < 64; ++i) __nanosleep(1000);
-      __syncwarp();
-    }
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;"
-                 ::"r"(tmem), "r"(PL_COLS)
-                 : "memory");
-  }
+  if (warp == 1) tc_release(tmem, PairColumns{PL_COLS}, ctl->abort_flag != 0);
 }
 
 // ----------------------------------------------------------------- host side

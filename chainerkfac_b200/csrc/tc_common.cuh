@@ -7,6 +7,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace kfac {
@@ -233,16 +235,23 @@ __device__ __forceinline__ void tc_ld_16x32(unsigned taddr, float v[16]) {
 // last barrier.  `aborted`: a wait of the block ran out, and the copies and MMAs
 // already issued get time to end before the tensor memory, and with the block its
 // shared memory, are another's (bounded: 64 us).  Not ahead of that barrier: a warp
-// that is done before the others wait would find no flag.
-__device__ __forceinline__ void tc_release(unsigned tmem, unsigned columns,
+// that is done before the others wait would find no flag.  `columns`: PairColumns
+// where a pair of blocks took them together (cta_group::2), by a warp of each.
+struct PairColumns {
+  unsigned n;
+  __device__ __forceinline__ operator unsigned() const { return n; }
+};
+template <typename Columns>
+__device__ __forceinline__ void tc_release(unsigned tmem, Columns columns,
                                            bool aborted) {
+  constexpr int kGroup = std::is_same<Columns, PairColumns>::value ? 2 : 1;
   if (aborted) {
 #pragma unroll 1
     for (int i = 0; i < 64; ++i) __nanosleep(1000);
     __syncwarp();
   }
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
-               ::"r"(tmem), "r"(columns)
+  asm volatile("tcgen05.dealloc.cta_group::%2.sync.aligned.b32 %0, %1;"
+               ::"r"(tmem), "r"((unsigned)columns), "n"(kGroup)
                : "memory");
 }
 

@@ -14,6 +14,8 @@ same face so the optimizer code reads like the reference's.
 import torch
 from torch import nn
 
+from chainerkfac_b200.embed_id import EmbedID as _EmbedIDModule
+
 
 class Parameter(object):
     """Chainer-style view of one ``torch.nn.Parameter``."""
@@ -160,6 +162,21 @@ class BatchNormalization(Link):
         return self.module.running_mean
 
 
+class EmbedID(Link):
+    """Chainer's ``EmbedID`` (``W``, ``ignore_label``), with a scale."""
+
+    param_names = (('W', 'weight'),)
+    b = None
+
+    @property
+    def ignore_label(self):
+        return self.module.ignore_label
+
+    @property
+    def scale(self):
+        return self.module.scale
+
+
 def _supported_conv(m):
     return (isinstance(m, nn.Conv2d) and m.groups == 1 and
             tuple(m.dilation) == (1, 1) and
@@ -181,6 +198,8 @@ def wrap(module):
         link = Convolution2D(module)
     elif isinstance(module, (nn.BatchNorm1d, nn.BatchNorm2d)) and module.affine:
         link = BatchNormalization(module)
+    elif isinstance(module, _EmbedIDModule):
+        link = EmbedID(module)
     else:
         link = Link(module)
         for name, child in module.named_children():

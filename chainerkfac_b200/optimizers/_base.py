@@ -67,6 +67,15 @@ class UpdateRule(object):
     def update(self, param):
         if not self.enabled:
             return
+        self.prepare(param)
+        for hook in self._pre_update_hooks.values():
+            hook(self, param)
+        self.update_core(param)
+        for hook in self._post_update_hooks.values():
+            hook(self, param)
+
+    def prepare(self, param):
+        """What comes before the hooks and ``update_core``."""
         self.t += 1
         if self._state is None:
             self._state = {}
@@ -76,11 +85,6 @@ class UpdateRule(object):
         if getattr(param, '_loss_scale', None) is not None and \
                 param.grad is not None:
             param.grad /= param._loss_scale
-        for hook in self._pre_update_hooks.values():
-            hook(self, param)
-        self.update_core(param)
-        for hook in self._post_update_hooks.values():
-            hook(self, param)
 
     def update_core(self, param):
         raise NotImplementedError

@@ -20,6 +20,7 @@ from torch import nn
 from chainerkfac_b200 import links as L
 from chainerkfac_b200 import ops
 from chainerkfac_b200.optimizers import _base
+from chainerkfac_b200.optimizers import orthogonal
 from chainerkfac_b200.optimizers import fisher_blocks as FB
 from chainerkfac_b200.optimizers.fisher_block import PI_TYPE_TRACENORM
 
@@ -38,6 +39,8 @@ def fblock_constructor(sub_linkname, sub_link, **kwargs):
         return FB.FisherBlockLinear(*args, **kwargs)
     elif isinstance(sub_link, L.Convolution2D):
         return FB.FisherBlockConvolution2D(*args, **kwargs)
+    elif isinstance(sub_link, L.EmbedID):
+        return FB.FisherBlockEmbedID(*args, **kwargs)
     elif isinstance(sub_link, L.BatchNormalization):
         if sub_link.gamma is None and sub_link.beta is None:
             return None
@@ -418,6 +421,7 @@ class KFAC(_base.GradientMethod):
             if fblock is None:
                 continue
             self.fblocks.append(fblock)
+        check_embeddings(self.fblocks)
         self._set_low_rank(1, 0, None)
         self.kfhook = KFACHook(self.fblocks)
         self._pre_hooked = False
@@ -610,7 +614,7 @@ class KFAC(_base.GradientMethod):
         self.update_kfgrads(self.fblocks)
 
         if not self.only_pic_update_weight:
-            for param in self.target.params():
+            for param in orthogonal.update_together(self.target.params()):
                 param.update()
 
         self.reallocate_cleared_grads()
@@ -885,6 +889,12 @@ class KFAC(_base.GradientMethod):
                     if part_bn:
                         self._precondition_bn(part_bn)
                     done.update(id(fb) for fb in part + part_bn)
+            k = 0
+            for fb in group:
+                # (an embedding's update reads what its plan adds to diagonals)
+                if isinstance(fb, FB.FisherBlockEmbedID):
+                    fb.set_diag_vals(plan.diag_items.at(k))
+                k += len(fb.plan_factors())
             pending = plan.run(damping, pi_type == PI_TYPE_TRACENORM,
                                after_class=after, join=not defer)
             if defer:
@@ -997,6 +1007,12 @@ class KFAC(_base.GradientMethod):
         lr = self.hyperparam.lr
         mom = None
         for fb in conn:
+            if isinstance(fb, FB.FisherBlockEmbedID):
+                self._precondition_embedding(fb)
+        conn = [fb for fb in conn if not isinstance(fb, FB.FisherBlockEmbedID)]
+        if not conn:
+            return
+        for fb in conn:
             W, b = fb.link.W, fb.link.b
             kfW, kfb = fb.kfgrad_buffers()
             Ai.append(fb.invs[0])
@@ -1026,6 +1042,17 @@ class KFAC(_base.GradientMethod):
                          ws_key=ws_key)
         for p in fused_params:
             p._kfac_applied = True
+
+
+    def _precondition_embedding(self, fb):
+        W = fb.link.W
+        if self._can_fuse(W):
+            rule = W.update_rule
+            fb.precondition(W.data, rule.velocity(W), self.hyperparam.lr,
+                            rule.effective_momentum())
+            W._kfac_applied = True
+        else:
+            fb.precondition()
 
 
 class DistributedKFAC(KFAC):
@@ -1237,9 +1264,26 @@ class DistributedKFAC(KFAC):
         return super(DistributedKFAC, self)._can_fuse(param)
 
 
+def check_embeddings(fblocks):
+    """An embedding's weight that another block updates too (an output layer
+    that shares it) would be updated twice."""
+    owner = {}
+    for fb in fblocks:
+        for param in fb.link.params():
+            other = owner.setdefault(id(param._p), fb)
+            if other is not fb and (
+                    isinstance(fb, FB.FisherBlockEmbedID) or
+                    isinstance(other, FB.FisherBlockEmbedID)):
+                raise ValueError(
+                    '%s and %s share a weight: give one of them no block '
+                    '(`constructor`)' % (other.linkname, fb.linkname))
+
+
 def block_cost(fblock):
     """Inverse cost of a block: sum of d^3 over its factors."""
     link = fblock.link
+    if isinstance(link, L.EmbedID):
+        return float(link.W.shape[1]) ** 3
     if hasattr(link, 'W'):
         dG = link.W.shape[0]
         dA = link.W.size // dG + (0 if link.b is None else 1)

@@ -18,6 +18,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "tc_common.cuh"
 
 namespace kfac {
 namespace {
@@ -75,14 +76,29 @@ struct alignas(V * sizeof(T)) Pack {
   T x[V];
 };
 
+// A word to memory, past the caches' other contents where what is written is more
+// than they hold anyway (STREAM).
+template <bool STREAM, typename P>
+__device__ __forceinline__ void put_word(P* to, const P& x) {
+  if constexpr (STREAM && sizeof(P) == 16) {
+    __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(&x));
+  } else {
+    *to = x;
+  }
+}
+constexpr long long kStreamBytes = 64LL << 20;      // half of the L2 cache
+
 // ------------------------------------------------------------------ lookup
 
-constexpr int kLookThreads = 256;
-constexpr int kLookRows = 4;      // rows a thread has in flight
+// 65536 tokens x 2048 bf16 over 128000: 66 us (a copy of as much takes 88), 70 with four
+// rows in flight; 72 with 128 threads, 88 with 256, 119 with 256, four rows and stores
+// that stay in the caches.
+constexpr int kLookThreads = 64;
+constexpr int kLookRows = 2;      // rows a thread has in flight
 
 // `lanes` threads (a power of two) share a row; a block has kLookThreads / lanes
 // rows at a time, kLookRows times.
-template <typename T, int V>
+template <typename T, int V, bool STREAM>
 __global__ void __launch_bounds__(kLookThreads)
 embed_lookup_kernel(const T* __restrict__ weight, const Ids ids, int width,
                     float scale, T* __restrict__ out, int lanes) {
@@ -115,7 +131,8 @@ embed_lookup_kernel(const T* __restrict__ weight, const Ids ids, int width,
         for (int e = 0; e < V; ++e)
           x[u].x[e] = Num<T>::put(row[u] >= 0 ? scale * Num<T>::get(x[u].x[e])
                                               : none);
-        *reinterpret_cast<P*>(out + i * width + (long long)w * V) = x[u];
+        put_word<STREAM>(reinterpret_cast<P*>(out + i * width + (long long)w * V),
+                         x[u]);
       }
     }
   }
@@ -197,52 +214,135 @@ __device__ __forceinline__ int sum_before(SortCounts& s, int x) {
   return front + inc - x;
 }
 
-// All passes of up to kSortTile tokens by one block.
-__global__ void __launch_bounds__(kSortThreads)
-token_sort_tile_kernel(const Ids ids, int bits, int passes, int* keys_out,
-                       int* perm_out) {
-  extern __shared__ unsigned char sort_smem[];
-  SortCounts& s = *reinterpret_cast<SortCounts*>(sort_smem);
-  int* keys = reinterpret_cast<int*>(sort_smem + sizeof(SortCounts));
-  unsigned short* perm = reinterpret_cast<unsigned short*>(keys + kSortTile);
+// All passes of up to 131072 tokens in one launch, by a cluster of up to sixteen blocks:
+// a block holds 1024 ITEMS keys, hands its counts to the others and puts every key
+// where it belongs in any block's shared memory.  65536 tokens of 128000: LATER.
+constexpr int kClusterThreads = 1024;
+constexpr int kClusterWarps = kClusterThreads / 32;
+constexpr int kClusterItems = 8;
+constexpr int kClusterMax = 16;
+constexpr int kClusterTokens = kClusterMax * kClusterThreads * kClusterItems;
+
+struct ClusterCounts {
+  unsigned short warp[kClusterWarps][kBins];
+  int total[kBins];
+  int base[kBins];
+  int part[kClusterWarps];
+};
+
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ unsigned in_block(const void* p, int block) {
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;"
+      : "=r"(r)
+      : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(block));
+  return r;
+}
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kClusterThreads)
+token_sort_cluster_kernel(const Ids ids, int bits, int passes, int* keys_out,
+                          int* perm_out) {
+  extern __shared__ __align__(16) unsigned char sort_smem[];
+  ClusterCounts& s = *reinterpret_cast<ClusterCounts*>(sort_smem);
+  int2* const data = reinterpret_cast<int2*>(sort_smem + sizeof(ClusterCounts));
+  constexpr int kTile = kClusterThreads * ITEMS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int first = warp * 32 * kSortItems + lane;
-  const int n = (int)ids.n;
-  int key[kSortItems], pos[kSortItems], rank[kSortItems];
+  const int blocks = gridDim.x, me = blockIdx.x;      // (the launch is one cluster)
+  const int first = warp * 32 * ITEMS + lane, n = (int)ids.n;
+  int key[ITEMS], pos[ITEMS], rank[ITEMS];
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    pos[j] = first + 32 * j;
+  for (int j = 0; j < ITEMS; ++j) {
+    pos[j] = me * kTile + first + 32 * j;
+    // (a key behind the end has all bits set: it stays behind all others)
     key[j] = pos[j] < n ? key_of(ids, pos[j]) : 0x7fffffff;
   }
   for (int pass = 0; pass < passes; ++pass) {
     const Digit d = {pass * bits, (1 << bits) - 1};
-    rank_keys(s, key, d, rank);
+    unsigned short* const mine = s.warp[warp];
+    for (int b = lane; b < kBins / 2; b += 32)
+      reinterpret_cast<unsigned*>(mine)[b] = 0;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const int digit = (key[j] >> d.shift) & d.mask;
+      const unsigned peers = __match_any_sync(0xffffffffu, digit);
+      const int before = mine[digit];
+      __syncwarp();
+      rank[j] = before + __popc(peers & ((1u << lane) - 1));
+      if (lane == 31 - __clz(peers))
+        mine[digit] = (unsigned short)(before + __popc(peers));
+      __syncwarp();
+    }
     __syncthreads();
-    const int mine = count_before(s);
-    s.base[threadIdx.x] = sum_before(s, mine);
+    if (threadIdx.x < kBins) {
+      int run = 0;
+#pragma unroll
+      for (int w = 0; w < kClusterWarps; ++w) {
+        const int c = s.warp[w][threadIdx.x];
+        s.warp[w][threadIdx.x] = (unsigned short)run;
+        run += c;
+      }
+      s.total[threadIdx.x] = run;
+    }
+    cluster_barrier();
+    int all = 0, before = 0;
+    if (threadIdx.x < kBins) {
+#pragma unroll
+      for (int c = 0; c < kClusterMax; ++c) {
+        if (c >= blocks) break;
+        int x;
+        asm volatile("ld.shared::cluster.s32 %0, [%1];"
+                     : "=r"(x)
+                     : "r"(in_block(&s.total[threadIdx.x], c)));
+        all += x;
+        before += c < me ? x : 0;
+      }
+    }
+    int inc = all;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) s.part[warp] = inc;
+    __syncthreads();
+    if (threadIdx.x < kBins) {
+      int front = 0;
+#pragma unroll
+      for (int w = 0; w < kBins / 32; ++w) front += w < warp ? s.part[w] : 0;
+      s.base[threadIdx.x] = front + inc - all + before;
+    }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kSortItems; ++j) {
+    for (int j = 0; j < ITEMS; ++j) {
       const int digit = (key[j] >> d.shift) & d.mask;
       const int to = s.base[digit] + s.warp[warp][digit] + rank[j];
-      keys[to] = key[j];
-      perm[to] = (unsigned short)pos[j];
+      asm volatile("st.shared::cluster.v2.s32 [%0], {%1, %2};"
+                   ::"r"(in_block(&data[to % kTile], to / kTile)), "r"(key[j]),
+                     "r"(pos[j])
+                   : "memory");
     }
-    __syncthreads();
+    cluster_barrier();
 #pragma unroll
-    for (int j = 0; j < kSortItems; ++j) {
-      key[j] = keys[first + 32 * j];
-      pos[j] = perm[first + 32 * j];
+    for (int j = 0; j < ITEMS; ++j) {
+      const int2 x = data[first + 32 * j];
+      key[j] = x.x;
+      pos[j] = x.y;
     }
-    __syncthreads();
   }
-  // (a key behind the end is larger than any other in every digit)
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j)
-    if (first + 32 * j < n) {
-      keys_out[first + 32 * j] = key[j];
-      perm_out[first + 32 * j] = pos[j];
+  for (int j = 0; j < ITEMS; ++j) {
+    const int i = me * kTile + first + 32 * j;
+    if (i < n) {
+      keys_out[i] = key[j];
+      perm_out[i] = pos[j];
     }
+  }
 }
 
 // Keys of a tile; those of the first pass come from the tokens themselves.
@@ -351,7 +451,7 @@ struct Grad {
   int add;               // onto the rows that are there
 };
 
-template <typename T, int V>
+template <typename T, int V, bool STREAM = false>
 __device__ __forceinline__ void put_row(T* out, const float (&acc)[V], float scale,
                                         bool add) {
   using P = Pack<T, V>;
@@ -361,13 +461,15 @@ __device__ __forceinline__ void put_row(T* out, const float (&acc)[V], float sca
   for (int e = 0; e < V; ++e)
     x.x[e] = Num<T>::put(add ? fmaf(scale, acc[e], Num<T>::get(x.x[e]))
                              : scale * acc[e]);
-  *reinterpret_cast<P*>(out) = x;
+  put_word<STREAM>(reinterpret_cast<P*>(out), x);
 }
 
-template <typename T, int V>
+template <typename T, int V, bool STREAM>
 __global__ void __launch_bounds__(kGradThreads)
-embed_grad_kernel(const Grad g, const T* __restrict__ gy, T* __restrict__ out) {
+embed_grad_kernel(const Grad g, const T* gy, T* out) {
   using P = Pack<T, V>;
+  let_next_launch_begin();
+  wait_for_launch_before();
   if (blockIdx.x >= g.chunk_blocks) {
     // rows of tokens that do not occur
     __shared__ unsigned clear;
@@ -384,16 +486,27 @@ embed_grad_kernel(const Grad g, const T* __restrict__ gy, T* __restrict__ out) {
       if (threadIdx.x == 0) clear = m;
     }
     __syncthreads();
+    // (rows next to each other as one piece of memory, whatever their width: 32003
+    // rows of 771 floats GRADODD)
     unsigned rows = clear;
-    P zero;
-#pragma unroll
-    for (int e = 0; e < V; ++e) zero.x[e] = Num<T>::put(0.f);
-    const int words = g.width / V;
     while (rows != 0) {
-      const int r = r0 + __ffs(rows) - 1;
-      rows &= rows - 1;
-      P* to = reinterpret_cast<P*>(out + (long long)r * g.width);
-      for (int w = threadIdx.x; w < words; w += kGradThreads) to[w] = zero;
+      const int r = __ffs(rows) - 1;
+      const unsigned run = ~(rows >> r);
+      const int many = run == 0 ? 32 - r : min(__ffs(run) - 1, 32 - r);
+      rows = r + many >= 32 ? 0 : rows & (~0u << (r + many));
+      char* to = reinterpret_cast<char*>(out + (long long)(r0 + r) * g.width);
+      const long long bytes = (long long)many * g.width * sizeof(T);
+      const int front = (int)min(bytes, (long long)(-reinterpret_cast<uintptr_t>(to) & 15));
+      const long long words = (bytes - front) >> 4;
+      uint4* const body = reinterpret_cast<uint4*>(to + front);
+      const int back = (int)(bytes - front - (words << 4));
+      const T none = Num<T>::put(0.f);
+      constexpr int S = sizeof(T);
+      if (S * (int)threadIdx.x < front) reinterpret_cast<T*>(to)[threadIdx.x] = none;
+      if (S * (int)threadIdx.x < back)
+        reinterpret_cast<T*>(body + words)[threadIdx.x] = none;
+      for (long long w = threadIdx.x; w < words; w += kGradThreads)
+        put_word<STREAM>(body + w, make_uint4(0, 0, 0, 0));
     }
     return;
   }
@@ -417,7 +530,7 @@ embed_grad_kernel(const Grad g, const T* __restrict__ gy, T* __restrict__ out) {
 #pragma unroll
       for (int e = 0; e < V; ++e) to[e] = acc[e];
     } else {
-      put_row<T, V>(out + (long long)cur * g.width + col, acc, g.scale, g.add);
+      put_row<T, V, STREAM>(out + (long long)cur * g.width + col, acc, g.scale, g.add);
     }
   };
   for (long long p = p0; p < p1 && cur != g.vocab; p += kGradAhead) {
@@ -448,18 +561,19 @@ embed_grad_kernel(const Grad g, const T* __restrict__ gy, T* __restrict__ out) {
   if (cur != g.vocab) leave(cur == behind);
 }
 
-// Tokens whose positions lie in several chunks: the sum of their parts, a quarter of
-// the chunks by each quarter of the block.
-constexpr int kJoinCols = 128;
+// Tokens whose positions lie in several chunks: the sum of their parts, in order, by
+// the block of the chunk where the token begins; four columns a thread.  (A block for
+// every 128 columns of a chunk, most of them with nothing to do, took 75 us for 65536
+// tokens x 2048, so JOIN.)
+constexpr int kJoinThreads = 512;
 template <typename T>
-__global__ void __launch_bounds__(4 * kJoinCols)
-embed_join_kernel(const Grad g, T* __restrict__ out, int slabs) {
-  __shared__ float sums[3][kJoinCols];
-  __shared__ long long end;
-  const long long chunk = blockIdx.x / slabs;
+__global__ void __launch_bounds__(kJoinThreads)
+embed_join_kernel(const Grad g, T* out) {
+  __shared__ long long s_end;
+  const long long chunk = blockIdx.x;
   const long long p0 = chunk * g.chunk, p1 = p0 + g.chunk;
-  // the token that begins in this chunk and goes on behind it, if there is one
   if (p1 >= g.n) return;
+  wait_for_launch_before();
   const int key = g.keys[p1];
   if (key == g.vocab || g.keys[p1 - 1] != key ||
       (p0 > 0 && g.keys[p0 - 1] == key))
@@ -470,28 +584,30 @@ embed_join_kernel(const Grad g, T* __restrict__ out, int slabs) {
       const long long mid = (lo + hi) >> 1;
       if (g.keys[mid] <= key) lo = mid + 1; else hi = mid;
     }
-    end = (lo - 1) / g.chunk + 1;        // first chunk without it
+    s_end = (lo - 1) / g.chunk + 1;      // first chunk without it
   }
   __syncthreads();
-  const int quarter = threadIdx.x / kJoinCols;
-  const int col = (int)(blockIdx.x - chunk * slabs) * kJoinCols +
-                  (threadIdx.x & (kJoinCols - 1));
-  const long long many = end - chunk;    // parts: this chunk's, then the others'
-  const long long each = (many + 3) / 4;
-  const long long c0 = chunk + quarter * each;
-  const long long c1 = min(c0 + each, end);
-  float sum = 0.f;
-  if (col < g.width) {
+  const long long end = s_end;
+  const float4* const part = reinterpret_cast<const float4*>(g.part);
+  const long long pitch = g.pitch >> 2;
+  for (int c = threadIdx.x; 4 * c < g.width; c += kJoinThreads) {
+    float4 sum = part[(2 * chunk + 1) * pitch + c];
 #pragma unroll 8
-    for (long long c = c0; c < c1; ++c)
-      sum += g.part[(2 * c + (c == chunk ? 1 : 0)) * g.pitch + col];
+    for (long long k = chunk + 1; k < end; ++k) {
+      const float4 x = part[2 * k * pitch + c];
+      sum.x += x.x;
+      sum.y += x.y;
+      sum.z += x.z;
+      sum.w += x.w;
+    }
+    const float all[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float acc[1] = {all[e]};
+      if (4 * c + e < g.width)
+        put_row<T, 1>(out + (long long)key * g.width + 4 * c + e, acc, g.scale, g.add);
+    }
   }
-  if (quarter > 0) sums[quarter - 1][threadIdx.x & (kJoinCols - 1)] = sum;
-  __syncthreads();
-  if (quarter > 0 || col >= g.width) return;
-  const float acc[1] = {sum + sums[0][threadIdx.x] + sums[1][threadIdx.x] +
-                        sums[2][threadIdx.x]};
-  put_row<T, 1>(out + (long long)key * g.width + col, acc, g.scale, g.add);
 }
 
 // ------------------------------------------------------------------ counts
@@ -586,10 +702,11 @@ int look_up(const void* weight, const Ids& ids, int width, float scale, void* ou
   while (lanes < kLookThreads && lanes * V < width) lanes *= 2;
   const long long rows = (long long)(kLookThreads / lanes) * kLookRows;
   const long long blocks = (ids.n + rows - 1) / rows;
-  embed_lookup_kernel<T, V>
-      <<<(unsigned)std::min<long long>(blocks, 1 << 20), kLookThreads, 0, st>>>(
-          static_cast<const T*>(weight), ids, width, scale, static_cast<T*>(out),
-          lanes);
+  const bool stream = ids.n * width * (long long)sizeof(T) > kStreamBytes;
+  auto* kernel = stream ? embed_lookup_kernel<T, V, true>
+                        : embed_lookup_kernel<T, V, false>;
+  kernel<<<(unsigned)std::min<long long>(blocks, 1 << 20), kLookThreads, 0, st>>>(
+      static_cast<const T*>(weight), ids, width, scale, static_cast<T*>(out), lanes);
   KFAC_LAUNCH_CHECK("embed_lookup_kernel");
   return KFAC_OK;
 }
@@ -612,6 +729,47 @@ struct SortPlan {
   size_t keys, counts;      // bytes of a spare key (and perm) array, of the counts
 };
 
+// (up to 2048 tokens by one block: a cluster's barriers take longer than its help)
+template <int ITEMS>
+int launch_sort(const Ids& s, const SortPlan& p, int blocks, int* keys, int* positions,
+                cudaStream_t st) {
+  const int smem = (int)sizeof(ClusterCounts) + kClusterThreads * ITEMS * 8;
+  if (smem > 48 * 1024)
+    KFAC_CUDA(cudaFuncSetAttribute(token_sort_cluster_kernel<ITEMS>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (blocks > 8)
+    KFAC_CUDA(cudaFuncSetAttribute(token_sort_cluster_kernel<ITEMS>,
+                                   cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kClusterThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  KFAC_CUDA(cudaLaunchKernelEx(&cfg, token_sort_cluster_kernel<ITEMS>, s, p.bits,
+                               p.passes, keys, positions));
+  KFAC_LAUNCH_CHECK("token_sort_cluster_kernel");
+  return KFAC_OK;
+}
+
+int sort_in_cluster(const Ids& s, const SortPlan& p, int* keys, int* positions,
+                    cudaStream_t st) {
+  constexpr int T = kClusterThreads;
+  if (s.n <= T) return launch_sort<1>(s, p, 1, keys, positions, st);
+  if (s.n <= 2 * T) return launch_sort<2>(s, p, 1, keys, positions, st);
+  if (s.n <= 8 * T) return launch_sort<1>(s, p, 8, keys, positions, st);
+  if (s.n <= 16 * T) return launch_sort<1>(s, p, 16, keys, positions, st);
+  if (s.n <= 32 * T) return launch_sort<2>(s, p, 16, keys, positions, st);
+  if (s.n <= 64 * T) return launch_sort<4>(s, p, 16, keys, positions, st);
+  return launch_sort<8>(s, p, 16, keys, positions, st);
+}
+
 SortPlan plan_sort(int64_t n, int64_t vocab) {
   SortPlan p;
   int need = 1;
@@ -619,8 +777,8 @@ SortPlan plan_sort(int64_t n, int64_t vocab) {
   p.passes = (need + kDigitBits - 1) / kDigitBits;
   p.bits = (need + p.passes - 1) / p.passes;
   p.tiles = (n + kSortTile - 1) / kSortTile;
-  p.keys = p.tiles > 1 ? ((size_t)n * 4 + 255) & ~(size_t)255 : 0;
-  p.counts = p.tiles > 1 ? (size_t)p.tiles * kBins * sizeof(int) : 0;
+  p.keys = n > kClusterTokens ? ((size_t)n * 4 + 255) & ~(size_t)255 : 0;
+  p.counts = n > kClusterTokens ? (size_t)p.tiles * kBins * sizeof(int) : 0;
   return p;
 }
 
@@ -639,7 +797,7 @@ GradPlan plan_grad(int64_t n, int width, int v) {
   p.slabs = (width + p.lanes * v - 1) / (p.lanes * v);
   p.chunk = 8;
   const long long per = kGradThreads / p.lanes;
-  while (p.chunk < 64 &&
+  while (p.chunk < 256 &&
          parts_of(parts_of(n, p.chunk) * p.slabs, per) > 16 * 148)
     p.chunk *= 2;
   p.chunks = parts_of(n, p.chunk);
@@ -660,15 +818,17 @@ int run_grad(Grad g, const void* gy, void* out, cudaStream_t st) {
   const long long blocks = g.chunk_blocks + clear;
   KFAC_REQUIRE(blocks < (1LL << 31), "embedding_grad: too many blocks");
   if (blocks == 0) return KFAC_OK;
-  embed_grad_kernel<T, V><<<(unsigned)blocks, kGradThreads, 0, st>>>(
-      g, static_cast<const T*>(gy), static_cast<T*>(out));
-  KFAC_LAUNCH_CHECK("embed_grad_kernel");
+  const bool stream =
+      !g.add && (long long)g.vocab * g.width * (long long)sizeof(T) > kStreamBytes;
+  auto* kernel = stream ? embed_grad_kernel<T, V, true> : embed_grad_kernel<T, V, false>;
+  const int rc = launch_behind("embed_grad_kernel", true, kernel, (int)blocks,
+                               kGradThreads, 0, st, g, static_cast<const T*>(gy),
+                               static_cast<T*>(out));
+  if (rc != KFAC_OK) return rc;
   if (p.chunks > 1) {
-    const int slabs = ceil_div(g.width, kJoinCols);
-    KFAC_REQUIRE(p.chunks * slabs < (1LL << 31), "embedding_grad: too many blocks");
-    embed_join_kernel<T><<<(unsigned)(p.chunks * slabs), 4 * kJoinCols, 0, st>>>(
-        g, static_cast<T*>(out), slabs);
-    KFAC_LAUNCH_CHECK("embed_join_kernel");
+    KFAC_REQUIRE(p.chunks < (1LL << 31), "embedding_grad: too many blocks");
+    return launch_behind("embed_join_kernel", true, embed_join_kernel<T>, (int)p.chunks,
+                         kJoinThreads, 0, st, g, static_cast<T*>(out));
   }
   return KFAC_OK;
 }
@@ -731,16 +891,7 @@ extern "C" int kfac_token_order(const void* ids, int id_bytes, int64_t n,
                "token_order: the workspace is not aligned to 4 bytes");
   const Ids s = make_ids(ids, id_bytes, n, vocab, has_ignore, ignore);
   cudaStream_t st = (cudaStream_t)stream;
-  if (p.tiles == 1) {
-    const int smem = (int)sizeof(SortCounts) + kSortTile * 6;
-    KFAC_CUDA(cudaFuncSetAttribute(token_sort_tile_kernel,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   smem));
-    token_sort_tile_kernel<<<1, kSortThreads, smem, st>>>(s, p.bits, p.passes, keys,
-                                                          positions);
-    KFAC_LAUNCH_CHECK("token_sort_tile_kernel");
-    return KFAC_OK;
-  }
+  if (n <= kClusterTokens) return sort_in_cluster(s, p, keys, positions, st);
   char* ws = static_cast<char*>(workspace);
   int* spare_keys = reinterpret_cast<int*>(ws);
   int* spare_perm = reinterpret_cast<int*>(ws + p.keys);

@@ -8,7 +8,10 @@
 // terms, scaled by its own power of two, into the next free row of the planes
 // (planes.cuh) that are multiplied by G_inv; which row of the planes makes no
 // difference to its values.  The second launch multiplies as many rows as there are,
-// and its epilogue scales, scatters and updates them.
+// and its epilogue scales and scatters them; the third updates their weights.  (In that
+// epilogue an SM has to store three rows where it now stores one, 32 bytes a cycle:
+// 32000 x 1024 with 12 800 rows reached 209 us so, STEP; 8000 x 256 with 300 rows, four
+// SMs at work, 36 us, SMALL.)
 //
 // Bound: HBM, 24 bytes an element (gradient in, kf out, velocity and weight in and
 // out), where the batch reaches few tokens; else the products, three MMAs each.
@@ -28,7 +31,7 @@ struct EmbedStep {
   const float* A;
   const float* damping;            // one value
   const float* grad;
-  float* kf;                       // or null
+  float* kf;
   float* param;                    // or null, with mom
   float* mom;
   float lr, momentum;
@@ -105,8 +108,7 @@ __device__ __forceinline__ void rest_row(const EmbedStep& e, long long at, int l
       for (int u = 0; u < 4; ++u) {
         const int k = k0 + 32 * u;
         if (k >= n) break;
-        if (e.kf != nullptr)
-          reinterpret_cast<float4*>(e.kf + at)[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        reinterpret_cast<float4*>(e.kf + at)[k] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (e.param == nullptr) continue;
         v[u].x *= e.momentum; v[u].y *= e.momentum;
         v[u].z *= e.momentum; v[u].w *= e.momentum;
@@ -119,7 +121,7 @@ __device__ __forceinline__ void rest_row(const EmbedStep& e, long long at, int l
   }
 #pragma unroll 4
   for (int k = lane; k < e.width; k += 32) {
-    if (e.kf != nullptr) e.kf[at + k] = 0.f;
+    e.kf[at + k] = 0.f;
     if (e.param == nullptr) continue;
     const float v = e.momentum * e.mom[at + k];
     e.mom[at + k] = v;
@@ -160,85 +162,125 @@ embed_rows_kernel(const __grid_constant__ EmbedStep e) {
 struct EpiEmbed {
   EmbedStep e;
 
+  // Of row `lane`: its token, exponent and divisor.
+  struct Row {
+    int token, exp;
+    float inv;
+  };
+  __device__ __forceinline__ Row begin(const PlaneFields& g, const PlaneTile& t) const {
+    Row o;
+    const int r = max(min(t.r0 + t.lane, g.M - 1), 0);
+    o.token = e.index[r];
+    o.exp = e.row_exp[r];
+    o.inv = 1.f / (e.A[o.token] + *e.damping);
+    return o;
+  }
+
   __device__ __forceinline__ void store(const PlaneFields& g, const PlaneTile& t,
-                                        float (&v)[32], bool) const {
+                                        float (&v)[32], bool, const Row& ahead) const {
     const unsigned piece = smem_u32(t.piece);
     const int lane = t.lane, width = e.width;
-    // of row `lane`
-    const int r = min(t.r0 + lane, g.M - 1);
-    const int token = e.index[r], re = e.row_exp[r];
-    const float inv = 1.f / (e.A[token] + *e.damping);
+    const int token = ahead.token, re = ahead.exp;
+    const float inv = ahead.inv;
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] *= g.gain;
     __syncwarp();
     pl_put_floats(piece, v, lane);
     __syncwarp();
     const int rows = min(32, g.M - t.r0);
-    const bool fused = e.param != nullptr;
     if (e.vec) {
       const int c = t.c0 + 4 * (lane & 7);
       const bool live = c < width;
-      int ce[4];
+      // (the array's end is padded to whole words)
+      const int4 ce = live ? *reinterpret_cast<const int4*>(e.col_exp + c)
+                           : make_int4(0, 0, 0, 0);
+      // Two factors, of the column and of the row, where neither they nor what is
+      // between them can leave the range; else exponents added up for every value.
+      const bool near = abs(re) <= 60 && inv >= 1e-18f && inv <= 1e18f &&
+                        max(max(abs(ce.x), abs(ce.y)), max(abs(ce.z), abs(ce.w))) <= 60;
+      if (__all_sync(0xffffffffu, near)) {
+        const float row_f = scale_exp(inv, re);
+        const float4 col_f =
+            make_float4(scale_exp(1.f, ce.x), scale_exp(1.f, ce.y),
+                        scale_exp(1.f, ce.z), scale_exp(1.f, ce.w));
 #pragma unroll
-      for (int k = 0; k < 4; ++k) ce[k] = live ? e.col_exp[c + k] : 0;
-#pragma unroll
-      for (int i0 = 0; i0 < 32; i0 += 8) {
-        float4 old_v[2], old_p[2];
-        long long at[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int row = i0 + 4 * u + (lane >> 3);
-          at[u] = (long long)__shfl_sync(0xffffffffu, token, row) * width + c;
-          if (fused && live && row < rows) {
-            old_v[u] = *reinterpret_cast<const float4*>(e.mom + at[u]);
-            old_p[u] = *reinterpret_cast<const float4*>(e.param + at[u]);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int row = i0 + 4 * u + (lane >> 3);
-          const int n = __shfl_sync(0xffffffffu, re, row);
-          const float f = __shfl_sync(0xffffffffu, inv, row);
-          if (!live || row >= rows) continue;
+        for (int i = 0; i < 32; i += 4) {
+          const int row = i + (lane >> 3);
+          const float f = __shfl_sync(0xffffffffu, row_f, row);
+          const int to = __shfl_sync(0xffffffffu, token, row);
           float4 x = pl_word(piece, row, lane & 7);
-          x.x = scale_exp(x.x, n + ce[0]) * f;
-          x.y = scale_exp(x.y, n + ce[1]) * f;
-          x.z = scale_exp(x.z, n + ce[2]) * f;
-          x.w = scale_exp(x.w, n + ce[3]) * f;
-          if (e.kf != nullptr) *reinterpret_cast<float4*>(e.kf + at[u]) = x;
-          if (!fused) continue;
-          float4 w = old_v[u];
-          w.x = e.momentum * w.x - e.lr * x.x;
-          w.y = e.momentum * w.y - e.lr * x.y;
-          w.z = e.momentum * w.z - e.lr * x.z;
-          w.w = e.momentum * w.w - e.lr * x.w;
-          *reinterpret_cast<float4*>(e.mom + at[u]) = w;
-          w.x += old_p[u].x;
-          w.y += old_p[u].y;
-          w.z += old_p[u].z;
-          w.w += old_p[u].w;
-          *reinterpret_cast<float4*>(e.param + at[u]) = w;
+          x.x *= col_f.x * f;
+          x.y *= col_f.y * f;
+          x.z *= col_f.z * f;
+          x.w *= col_f.w * f;
+          if (live && row < rows)
+            *reinterpret_cast<float4*>(e.kf + (long long)to * width + c) = x;
         }
+        return;
       }
-      return;
     }
     const int c = t.c0 + lane;
     const int ce = c < width ? e.col_exp[c] : 0;
 #pragma unroll 4
     for (int row = 0; row < rows; ++row) {
-      const long long at = (long long)__shfl_sync(0xffffffffu, token, row) * width + c;
+      const int to = __shfl_sync(0xffffffffu, token, row);
       const int n = __shfl_sync(0xffffffffu, re, row);
       const float f = __shfl_sync(0xffffffffu, inv, row);
-      if (c >= width) continue;
       const float x = scale_exp(pl_float(piece, row, lane), n + ce) * f;
-      if (e.kf != nullptr) e.kf[at] = x;
-      if (!fused) continue;
-      const float w = e.momentum * e.mom[at] - e.lr * x;
-      e.mom[at] = w;
-      e.param[at] += w;
+      if (c < width) e.kf[(long long)to * width + c] = x;
     }
   }
 };
+
+// The momentum update of the rows that have a gradient, a row a warp.
+__global__ void __launch_bounds__(kThreads)
+embed_update_kernel(const __grid_constant__ EmbedStep e) {
+  wait_for_launch_before();
+  const int lane = threadIdx.x & 31;
+  const int rows = *reinterpret_cast<const volatile int*>(e.count);
+  for (int r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < rows;
+       r += gridDim.x * kWarps) {
+    const long long at = (long long)e.index[r] * e.width;
+    if (e.vec) {
+      const int n = e.width >> 2;
+#pragma unroll 1
+      for (int k0 = lane; k0 < n; k0 += 128) {
+        float4 x[4], v[4], p[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int k = min(k0 + 32 * u, n - 1);
+          x[u] = reinterpret_cast<const float4*>(e.kf + at)[k];
+          v[u] = reinterpret_cast<const float4*>(e.mom + at)[k];
+          p[u] = reinterpret_cast<const float4*>(e.param + at)[k];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int k = k0 + 32 * u;
+          if (k >= n) break;
+          v[u].x = e.momentum * v[u].x - e.lr * x[u].x;
+          v[u].y = e.momentum * v[u].y - e.lr * x[u].y;
+          v[u].z = e.momentum * v[u].z - e.lr * x[u].z;
+          v[u].w = e.momentum * v[u].w - e.lr * x[u].w;
+          reinterpret_cast<float4*>(e.mom + at)[k] = v[u];
+          p[u].x += v[u].x;
+          p[u].y += v[u].y;
+          p[u].z += v[u].z;
+          p[u].w += v[u].w;
+          reinterpret_cast<float4*>(e.param + at)[k] = p[u];
+        }
+      }
+      continue;
+    }
+#pragma unroll 4
+    for (int k = lane; k < e.width; k += 32) {
+      const float v = e.momentum * e.mom[at + k] - e.lr * e.kf[at + k];
+      e.mom[at + k] = v;
+      e.param[at + k] += v;
+    }
+  }
+}
+
+long long parts_of(long long a, long long b) { return (a + b - 1) / b; }
 
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
@@ -305,12 +347,10 @@ extern "C" int kfac_precondition_embedding(int64_t vocab, int width, const float
   int rc = check_shape(vocab, width);
   if (rc != KFAC_OK) return rc;
   KFAC_REQUIRE(G_inv != nullptr && A != nullptr && damping != nullptr &&
-                   grad != nullptr,
+                   grad != nullptr && kf != nullptr,
                "precondition_embedding: null pointer");
   KFAC_REQUIRE((param == nullptr) == (mom == nullptr),
                "precondition_embedding: a weight and its velocity go together");
-  KFAC_REQUIRE(kf != nullptr || param != nullptr,
-               "precondition_embedding: nowhere to go");
   const size_t need = lay_out(vocab, width, nullptr, nullptr);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(KFAC_ERR_WORKSPACE,
@@ -338,7 +378,7 @@ extern "C" int kfac_precondition_embedding(int64_t vocab, int width, const float
   cudaStream_t st = (cudaStream_t)stream;
   KFAC_CUDA(cudaMemsetAsync(e.count, 0, sizeof(int), st));
   const long long rows = vocab + width;
-  embed_rows_kernel<<<(unsigned)std::min<long long>((rows + kWarps - 1) / kWarps,
+  embed_rows_kernel<<<(unsigned)std::min<long long>(parts_of(rows, kWarps),
                                                     (long long)sm_count() * 8),
                       kThreads, 0, st>>>(e);
   KFAC_LAUNCH_CHECK("embed_rows_kernel");
@@ -354,5 +394,10 @@ extern "C" int kfac_precondition_embedding(int64_t vocab, int width, const float
     return rc;
   plane_number_tiles(l);
   l.rows = e.count;
-  return plane_launch("embed products", l, EpiEmbed{e}, true, st);
+  rc = plane_launch("embed products", l, EpiEmbed{e}, true, st);
+  if (rc != KFAC_OK || param == nullptr) return rc;
+  return launch_behind("embed_update_kernel", true, embed_update_kernel,
+                       (int)std::min<long long>(parts_of(vocab, kWarps),
+                                                (long long)sm_count() * 8),
+                       kThreads, 0, st, e);
 }

@@ -175,8 +175,13 @@ struct EpiPlanes {
   float alpha, beta, diag;
   int terms;
   bool poly;
+  __device__ __forceinline__ NothingAhead begin(const PlaneFields&,
+                                                const PlaneTile&) const {
+    return NothingAhead();
+  }
   __device__ __forceinline__ void store(const PlaneFields& g, const PlaneTile& t,
-                                        float (&v)[32], bool mirror) const {
+                                        float (&v)[32], bool mirror,
+                                        NothingAhead) const {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] *= alpha * g.gain;
     if (poly) {
@@ -237,8 +242,12 @@ struct EpiPlanes {
 template <typename T>
 struct EpiLast {
   float alpha, keep, lr;
+  __device__ __forceinline__ NothingAhead begin(const PlaneFields&,
+                                                const PlaneTile&) const {
+    return NothingAhead();
+  }
   __device__ __forceinline__ void store(const PlaneFields& g, const PlaneTile& t,
-                                        float (&v)[32], bool) const {
+                                        float (&v)[32], bool, NothingAhead) const {
     const unsigned piece = smem_u32(t.piece);
     T* const dst = static_cast<T*>(g.dst);
     T* const param = static_cast<T*>(g.param);

@@ -223,6 +223,9 @@ __device__ __forceinline__ void ld_matrix(unsigned addr, unsigned& a, unsigned& 
                : "memory");
 }
 
+// For epilogues with nothing to do ahead.
+struct NothingAhead {};
+
 // 32 rows of 64 bytes in shared memory, without bank conflicts: 16-byte word j of a row.
 __device__ __forceinline__ int row64_off(int row, int j) {
   return row * 64 + ((j ^ ((row >> 1) & 3)) << 4);
@@ -349,8 +352,9 @@ __device__ __forceinline__ void pl_tile_at(const PlaneFields& g, int tile, int& 
   n0 = bj * PL_TILE;
 }
 
-// Epi: the epilogue's type; epi.store(problem, tile, v, mirror) takes the sums of a
-// PlaneTile, unscaled.
+// Epi: the epilogue's type.  epi.begin(problem, tile) is called for a warp's rows and
+// its first columns before the sums are there; epi.store(problem, tile, v, mirror,
+// what begin gave) takes the sums of a PlaneTile, unscaled.
 template <int N, typename Epi>
 __global__ void __launch_bounds__(PL_THREADS, 1)
 plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
@@ -548,6 +552,8 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
       t.r0 = m0 + PL_ROWS * side + 32 * q;
       const bool mirror = g.lower && m0 != n0;
       const int nseg = cut ? (nkb + PL_SEGMENT - 1) / PL_SEGMENT : (nkb > 0 ? 1 : 0);
+      t.c0 = n0 + 128 * h;
+      const auto ahead = epi.begin(g, t);
       float v[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) v[i] = 0.f;
@@ -617,7 +623,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
             }
           }
           t.c0 = n0 + part * width + c0;
-          if (t.r0 < g.M && t.c0 < g.N) epi.store(g, t, x, mirror);
+          if (t.r0 < g.M && t.c0 < g.N) epi.store(g, t, x, mirror, ahead);
         }
         break;
       }
@@ -628,7 +634,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
         float x[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[i] = v[32 * u + i];
-        if (t.r0 < g.M && t.c0 < g.N) epi.store(g, t, x, mirror);
+        if (t.r0 < g.M && t.c0 < g.N) epi.store(g, t, x, mirror, ahead);
       }
     }
   }

@@ -815,11 +815,12 @@ def _chk_ids(ids):
         raise ValueError('ids must be contiguous')
 
 
-def _chk_place(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError('%s is on %s, not on %s' % (name, t.device,
-                                                         device))
+def _chk_place(index, *tensors):
+    """(Names and) tensors that must be on the CUDA device `index`."""
+    for name, t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError('%s is on device %s, not on %d' % (
+                name, t.get_device(), index))
 
 
 def _chk_shape(t, shape, name):
@@ -845,23 +846,24 @@ def embedding(weight, ids, scale=1.0, ignore_label=None, out=None):
     _chk_ids(ids)
     if weight.dim() != 2:
         raise ValueError('weight must have two dimensions')
-    device = weight.device
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    index = weight.get_device()
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return embedding(weight, ids, scale, ignore_label, out)
     vocab, width = weight.shape
     shape = ids.shape + (width,)
     if out is None:
-        out = torch.empty(shape, dtype=weight.dtype, device=device)
+        out = weight.new_empty(shape)
     else:
         _chk_rows(out, 'out', (weight.dtype,))
         _chk_shape(out, shape, 'out')
-    _chk_place(device, ids=ids, out=out)
+        _chk_place(index, ('out', out))
+    _chk_place(index, ('ids', ids))
     has, label = _ignore(ignore_label)
     _lib.check(_lib.load().kfac_embedding(
         WIRE_DTYPES[weight.dtype], weight.data_ptr(), vocab, width,
         ids.data_ptr(), ids.element_size(), ids.numel(), has, label, scale,
-        out.data_ptr(), _stream()), 'kfac_embedding')
+        out.data_ptr(), _raw_stream(index)), 'kfac_embedding')
     return out
 
 
@@ -872,27 +874,45 @@ class TokenOrder(object):
 
     def __init__(self, ids, vocab, ignore_label=None):
         _chk_ids(ids)
-        self.device, self.vocab = ids.device, int(vocab)
+        self.index, self.vocab = ids.get_device(), int(vocab)
         self.count = ids.numel()
-        with torch.cuda.device(self.device):
-            lib = _lib.load()
-            self.keys, self.positions = torch.empty(
-                (2, self.count), dtype=torch.int32,
-                device=self.device).unbind(0)
-            ws = _scratch(lib.kfac_token_order_workspace_bytes(
-                self.count, self.vocab), self.device)
-            self.stream = _stream()
-            has, label = _ignore(ignore_label)
-            _lib.check(lib.kfac_token_order(
-                ids.data_ptr(), ids.element_size(), self.count, self.vocab,
-                has, label, self.keys.data_ptr(), self.positions.data_ptr(),
-                ws.data_ptr(), ws.numel(), self.stream), 'kfac_token_order')
+        if self.index != torch.cuda.current_device():
+            with torch.cuda.device(self.index):
+                self._sort(ids, ignore_label)
+        else:
+            self._sort(ids, ignore_label)
 
-    def used_here(self):
+    def _sort(self, ids, ignore_label):
+        lib = _lib.load()
+        n = self.count
+        # (keys, then positions)
+        self.sorted = ids.new_empty(2 * n, dtype=torch.int32)
+        self.stream = _raw_stream(self.index)
+        nbytes, ws = lib.kfac_token_order_workspace_bytes(n, self.vocab), None
+        if nbytes:
+            ws = ids.new_empty(nbytes, dtype=torch.uint8)
+        has, label = _ignore(ignore_label)
+        at = self.sorted.data_ptr()
+        _lib.check(lib.kfac_token_order(
+            ids.data_ptr(), ids.element_size(), n, self.vocab, has, label, at,
+            at + 4 * n, _p(ws), nbytes, self.stream), 'kfac_token_order')
+
+    @property
+    def keys(self):
+        return self.sorted[:self.count]
+
+    @property
+    def positions(self):
+        return self.sorted[self.count:]
+
+    def get_device(self):
+        return self.index
+
+    def used_on(self, stream):
         """Keeps the sorted positions from being handed out again while the
         current stream reads them, where that is another than theirs."""
-        if _stream() != self.stream:
-            self.keys.record_stream(torch.cuda.current_stream())
+        if stream != self.stream:
+            self.sorted.record_stream(torch.cuda.current_stream())
 
 
 def embedding_grad(gy, order, scale=1.0, out=None, accumulate=False):
@@ -907,28 +927,30 @@ def embedding_grad(gy, order, scale=1.0, out=None, accumulate=False):
     if gy.numel() != order.count * width:
         raise ValueError('gy must have a row for each of the %d tokens, got %s'
                          % (order.count, tuple(gy.shape)))
-    device = gy.device
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    index = gy.get_device()
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return embedding_grad(gy, order, scale, out, accumulate)
     shape = (order.vocab, width)
     if out is None:
         if accumulate:
             raise ValueError('accumulate needs an existing `out`')
-        out = torch.empty(shape, dtype=gy.dtype, device=device)
+        out = gy.new_empty(shape)
     else:
         _chk_rows(out, 'out', (gy.dtype,))
         _chk_shape(out, shape, 'out')
-    _chk_place(device, order=order, out=out)
+    _chk_place(index, ('order', order), ('out', out))
     lib = _lib.load()
-    ws = _scratch(lib.kfac_embedding_grad_workspace_bytes(order.count, width),
-                  device)
-    order.used_here()
+    n = order.count
+    nbytes = lib.kfac_embedding_grad_workspace_bytes(n, width)
+    ws = gy.new_empty(max(nbytes, 16), dtype=torch.uint8)
+    stream = _raw_stream(index)
+    order.used_on(stream)
+    at = order.sorted.data_ptr()
     _lib.check(lib.kfac_embedding_grad(
-        WIRE_DTYPES[gy.dtype], gy.data_ptr(), width, order.keys.data_ptr(),
-        order.positions.data_ptr(), order.count, order.vocab, scale,
-        int(bool(accumulate)), out.data_ptr(), ws.data_ptr(), ws.numel(),
-        _stream()), 'kfac_embedding_grad')
+        WIRE_DTYPES[gy.dtype], gy.data_ptr(), width, at, at + 4 * n, n,
+        order.vocab, scale, int(bool(accumulate)), out.data_ptr(),
+        ws.data_ptr(), nbytes, stream), 'kfac_embedding_grad')
     return out
 
 
@@ -953,7 +975,7 @@ def token_counts(ids, vocab, ignore_label=None, alpha=1.0, beta=0.0, out=None,
         _chk(mean, 'mean')
         if mean.numel() != 1:
             raise ValueError('mean must have one element')
-    _chk_place(device, out=out, mean=mean)
+    _chk_place(device.index, ('out', out), ('mean', mean))
     lib = _lib.load()
     ws = _scratch(lib.kfac_token_counts_workspace_bytes(vocab), device)
     has, label = _ignore(ignore_label)
@@ -991,8 +1013,8 @@ def precondition_embedding(G_inv, A, damping, grad, kf=None, param=None,
     for t, name in ((kf, 'kf'), (param, 'param'), (mom, 'mom')):
         if t is not None:
             _chk_shape(t, (vocab, width), name)
-    _chk_place(device, G_inv=G_inv, A=A, damping=damping, kf=kf, param=param,
-               mom=mom)
+    _chk_place(device.index, ('G_inv', G_inv), ('A', A), ('damping', damping),
+               ('kf', kf), ('param', param), ('mom', mom))
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return precondition_embedding(G_inv, A, damping, grad, kf, param,
@@ -1067,7 +1089,7 @@ def orthogonalize(xs, outs=None, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7,
             if t is not None:
                 _chk_rows(t, name, (x.dtype,))
                 _chk_shape(t, x.shape, name)
-        _chk_place(device, x=x, out=out, param=w)
+        _chk_place(device.index, ('x', x), ('out', out), ('param', w))
         groups.setdefault(x.dtype, []).append(i)
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):

@@ -574,7 +574,7 @@ int kfac_orthogonalize(int dtype, int count, const int* rows, const int* cols,
  * symmetric matrix, and `damping` one device float (the value that the inverse
  * plan added to the diagonal of A's place).  With a weight and its velocity,
  *     mom = momentum * mom - lr * kf,   param = param + mom.
- * kf or the pair may be NULL.  All fp32, dense, row-major.  Rows whose gradient
+ * The pair may be NULL.  All fp32, dense, row-major.  Rows whose gradient
  * is zero have kf = 0 and cost no product; one with values that are not finite
  * gives NaN in its own row. */
 size_t kfac_precondition_embedding_workspace_bytes(int64_t vocab, int width);

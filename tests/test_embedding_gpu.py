@@ -119,8 +119,8 @@ def test_lookup_leaves_what_is_behind_its_rows():
         assert (buf[:offset] == 9).all() and (buf[offset + 5 * width:] == 9).all()
 
 
-@pytest.mark.parametrize('n', [1, 2, 31, 33, 512, 4095, 4096, 4097, 9000,
-                               65537, 300001])
+@pytest.mark.parametrize('n', [1, 2, 31, 33, 512, 1025, 2049, 4097, 9000, 20000,
+                               65537, 131072, 131073, 300001])
 @pytest.mark.parametrize('vocab', [1, 2, 511, 512, 50021, 300000])
 def test_order_is_a_stable_sort(n, vocab):
     from chainerkfac_b200 import ops

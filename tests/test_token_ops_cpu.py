@@ -45,7 +45,7 @@ def test_embedding_calls_are_checked(lib):
 
 def test_token_orders_and_gradients_are_checked(lib):
     order = lambda **k: lib.kfac_token_order(*({**dict(
-        ids=FAKE, id_bytes=4, n=5000, vocab=10, has=0, ignore=0, keys=FAKE,
+        ids=FAKE, id_bytes=4, n=500000, vocab=10, has=0, ignore=0, keys=FAKE,
         positions=FAKE, ws=FAKE, nbytes=1 << 30, stream=None), **k}).values())
     assert order(id_bytes=3) == 1 and order(keys=None) == 1
     assert order(ws=None) == 3 and order(nbytes=100) == 3
@@ -67,9 +67,9 @@ def test_token_orders_and_gradients_are_checked(lib):
 
 
 def test_workspaces_of_the_sort_and_the_gradient(lib):
-    # one block sorts up to 4096 tokens without any
-    assert lib.kfac_token_order_workspace_bytes(4096, 50000) == 0
-    assert lib.kfac_token_order_workspace_bytes(4097, 50000) >= 2 * 4 * 4097
+    # one launch sorts up to 131072 tokens without any
+    assert lib.kfac_token_order_workspace_bytes(131072, 50000) == 0
+    assert lib.kfac_token_order_workspace_bytes(131073, 50000) >= 2 * 4 * 131073
     assert lib.kfac_token_order_workspace_bytes(-1, 5) == 0
     # two partial rows a chunk of at least eight positions
     for n, width in ((1, 1), (100, 33), (70000, 2048), (2 ** 31 - 5000, 8)):

@@ -60,6 +60,7 @@ int diag_status_read(int* out);
 
 // Status word of the orthogonalisation's products (ortho.cu).
 int ortho_status_read(int* out);
+int ortho_small_status_read(int* out);
 
 // And of an embedding's (embed_precond.cu).
 int embed_status_read(int* out);

@@ -24,16 +24,15 @@
 #include <exception>
 #include <vector>
 
+#include "ortho.cuh"
 #include "planes.cuh"
 
 namespace kfac {
 namespace {
 
-constexpr int kXExp = 13, kAExp = 12;
 constexpr int kNormThreads = 256;
 constexpr int kNormBlocksMax = 512;      // partial sums of a matrix
 constexpr long long kNormChunk = 8192;   // elements of a partial sum, at least
-constexpr int kStepsMax = 64;
 // Matrices of one row of launches, whose tables travel as kernel arguments (nothing
 // to copy, nothing to keep for a captured graph): up to 4 KB, or up to 32 KB.
 constexpr int kFew = 4, kMany = 40;
@@ -376,6 +375,38 @@ int launch_norm(const NormLaunch<N>& l, int norm_blocks, int pack_blocks,
                        kNormThreads, 0, st, l);
 }
 
+// Whether every matrix is one that a block orthogonalises by itself.  Beside larger
+// ones they ride along in the products' launches, which take no longer for them.
+bool all_small(int count, const int* rows, const int* cols) {
+  for (int i = 0; i < count; ++i)
+    if (std::min(rows[i], cols[i]) > kSmallShort ||
+        std::max(rows[i], cols[i]) > kSmallLong)
+      return false;
+  return true;
+}
+
+int run_small(int count, const int* rows, const int* cols, const Call& c,
+              void* stream) {
+  SmallLaunch l;
+  l.steps = c.steps;
+  l.eps = c.eps;
+  l.keep = 1.f - c.lr * c.decay;
+  l.lr = c.lr;
+  std::copy(c.coefficients, c.coefficients + 3 * c.steps, l.coefficients);
+  for (int first = 0; first < count; first += kSmallJobs) {
+    l.n = std::min(kSmallJobs, count - first);
+    for (int k = 0; k < l.n; ++k) {
+      const int i = first + k;
+      l.j[k] = {c.x[i], c.out != nullptr ? c.out[i] : nullptr,
+                c.param != nullptr ? c.param[i] : nullptr, rows[i], cols[i],
+                c.scale[i]};
+    }
+    const int rc = launch_ortho_small(l, c.dtype, (cudaStream_t)stream);
+    if (rc != KFAC_OK) return rc;
+  }
+  return KFAC_OK;
+}
+
 // All launches of up to N matrices, numbers first .. first + n of the call.
 template <int N>
 int run_group(const Shape* s, int first, int n, double* part, const Call& c,
@@ -559,6 +590,7 @@ extern "C" int kfac_orthogonalize(int dtype, int count, const int* rows,
     shapes.reserve(count);
     lay_out(count, rows, cols, ws, &shapes);
     const Call c = {dtype, steps, coefficients, eps, lr, decay, x, out, param, scale};
+    if (all_small(count, rows, cols)) return run_small(count, rows, cols, c, stream);
     double* part = reinterpret_cast<double*>(ws);
     cudaStream_t st = (cudaStream_t)stream;
     for (int i = 0; i < count;) {

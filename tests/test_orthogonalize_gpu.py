@@ -60,7 +60,10 @@ def check(got, x, want=None, **kw):
 
 SHAPES = [(1, 1), (1, 9), (7, 1), (2, 3), (16, 16), (31, 200), (64, 147),
           (127, 129), (128, 128), (129, 128), (255, 130), (300, 77),
-          (513, 512), (64, 1500), (1500, 200), (700, 1100)]
+          (513, 512), (64, 1500), (1500, 200), (700, 1100),
+          # what a block does by itself, turned and not, up to its sides
+          (147, 64), (256, 128), (128, 256), (256, 33), (33, 255), (257, 128),
+          (128, 257), (129, 129), (48, 49), (90, 17)]
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16,
@@ -104,6 +107,35 @@ def test_many_matrices_at_once(count):
         check(y.float() / s, x)
         # (alone a long sum may be cut elsewhere: near, not the same bits)
         assert torch.equal(y, z)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('count', [3, 70])
+def test_many_small_matrices(count, dtype):
+    """As many blocks as matrices; alone each gives the same bits."""
+    from chainerkfac_b200 import ops
+    g = gen(count)
+    xs = [torch.randn((1 + 37 * i % 128, 1 + 91 * i % 256)[::1 - 2 * (i % 2)],
+                      device='cuda', generator=g).to(dtype)
+          for i in range(count)]
+    got = ops.orthogonalize(xs, scale=[0.5 + i for i in range(count)])
+    for i, (x, y) in enumerate(zip(xs, got)):
+        check(y.float() / (0.5 + i), x)
+        assert torch.equal(y, ops.orthogonalize(x, scale=0.5 + i))
+
+
+@pytest.mark.parametrize('shape', [(60, 200), (200, 60)])
+def test_small_weights_are_updated_in_either_direction(shape):
+    from chainerkfac_b200 import ops
+    x = torch.randn(shape, device='cuda', generator=gen(1))
+    w = torch.randn(shape, device='cuda', generator=gen(2))
+    old, out = w.double(), torch.empty_like(x)
+    ops.orthogonalize(x, outs=out, params=w, lr=0.1, decay=0.3, scale=2.0)
+    step = 0.1 * 2.0 * reference(x)
+    off = float((w.double() - (1 - 0.03) * old + step).norm())
+    assert off <= tolerance(x) * float(step.norm()) + \
+        2.0 ** -23 * float(old.norm())
+    check(out / 2.0, x)
 
 
 def test_steps_coefficients_and_eps():

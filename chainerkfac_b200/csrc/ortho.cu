@@ -329,9 +329,20 @@ int norm_blocks_of(long long count) {
       1, std::min<long long>(kNormBlocksMax, (count + kNormChunk - 1) / kNormChunk));
 }
 
+// Whether every matrix is one that a block orthogonalises by itself.  Beside larger
+// ones they ride along in the products' launches, which take no longer for them.
+bool all_small(int count, const int* rows, const int* cols) {
+  for (int i = 0; i < count; ++i)
+    if (std::min(rows[i], cols[i]) > kSmallShort ||
+        std::max(rows[i], cols[i]) > kSmallLong)
+      return false;
+  return true;
+}
+
 // Lays the matrices' planes out behind `ws`; the bytes they take.
 size_t lay_out(int count, const int* rows, const int* cols, char* ws,
                std::vector<Shape>* shapes) {
+  if (all_small(count, rows, cols)) return 0;
   size_t at = 0;
   long long parts = 0;
   for (int i = 0; i < count; ++i)
@@ -373,16 +384,6 @@ int launch_norm(const NormLaunch<N>& l, int norm_blocks, int pack_blocks,
   KFAC_LAUNCH_CHECK("ortho_norm_kernel");
   return launch_behind("ortho_pack_kernel", true, ortho_pack_kernel<N, T>, pack_blocks,
                        kNormThreads, 0, st, l);
-}
-
-// Whether every matrix is one that a block orthogonalises by itself.  Beside larger
-// ones they ride along in the products' launches, which take no longer for them.
-bool all_small(int count, const int* rows, const int* cols) {
-  for (int i = 0; i < count; ++i)
-    if (std::min(rows[i], cols[i]) > kSmallShort ||
-        std::max(rows[i], cols[i]) > kSmallLong)
-      return false;
-  return true;
 }
 
 int run_small(int count, const int* rows, const int* cols, const Call& c,
@@ -579,6 +580,8 @@ extern "C" int kfac_orthogonalize(int dtype, int count, const int* rows,
                                      (param != nullptr && param[i] != nullptr)),
                  "orthogonalize: matrix %d is null, or has nowhere to go", i);
   try {
+    const Call c = {dtype, steps, coefficients, eps, lr, decay, x, out, param, scale};
+    if (all_small(count, rows, cols)) return run_small(count, rows, cols, c, stream);
     const size_t need = lay_out(count, rows, cols, nullptr, nullptr);
     if (workspace == nullptr || workspace_bytes < need)
       return fail(KFAC_ERR_WORKSPACE,
@@ -589,8 +592,6 @@ extern "C" int kfac_orthogonalize(int dtype, int count, const int* rows,
     std::vector<Shape> shapes;
     shapes.reserve(count);
     lay_out(count, rows, cols, ws, &shapes);
-    const Call c = {dtype, steps, coefficients, eps, lr, decay, x, out, param, scale};
-    if (all_small(count, rows, cols)) return run_small(count, rows, cols, c, stream);
     double* part = reinterpret_cast<double*>(ws);
     cudaStream_t st = (cudaStream_t)stream;
     for (int i = 0; i < count;) {

@@ -21,7 +21,7 @@
 namespace kfac {
 namespace {
 
-constexpr int OS_THREADS = 256;
+constexpr int OS_THREADS = 512;
 constexpr int OS_WARPS = OS_THREADS / 32;
 constexpr int OS_PLANE = 128 * 128;          // bytes: 128 rows of 64 fp16
 constexpr int OS_TILE = 2 * OS_PLANE;        // hi, lo
@@ -245,7 +245,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
     const float make_a = exp2f(kAExp - 2 * kXExp) * gain(ck);
     if (r0 < r) {
 #pragma unroll 1
-      for (int c0 = 32 * h; c0 < r; c0 += 64) {
+      for (int c0 = 32 * h; c0 < r; c0 += 32 * OS_WARPS / 4) {
         float v[32];
         os_sums(quarter + c0, 2 * terms - 1, 128, v);
 #pragma unroll
@@ -271,7 +271,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
     const float square = k3[2] * exp2f(-kAExp) * gain(nk), diag = k3[0] * exp2f(kAExp);
     if (r0 < r) {
 #pragma unroll 1
-      for (int c0 = 32 * h; c0 < r; c0 += 64) {
+      for (int c0 = 32 * h; c0 < r; c0 += 32 * OS_WARPS / 4) {
         float v[32];
         os_sums(quarter + c0, 2 * terms - 1, 128, v);
 #pragma unroll
@@ -309,7 +309,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
         exp2f(last ? -(kXExp + kAExp) : -kAExp) * gain(nk) * (last ? job.scale : 1.f);
     if (r0 >= r) continue;
 #pragma unroll 1
-    for (int c0 = 32 * h; c0 < c; c0 += 64) {
+    for (int c0 = 32 * h; c0 < c; c0 += 32 * OS_WARPS / 4) {
       float v[32];
       os_sums(quarter + c0, 2, 256, v);
 #pragma unroll

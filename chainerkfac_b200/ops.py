@@ -7,6 +7,7 @@ library's kernels.
 """
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -1038,14 +1039,21 @@ def precondition_embedding(G_inv, A, damping, grad, kf=None, param=None,
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
 
+@functools.lru_cache(maxsize=64)
+def _coefficient_array(rows):
+    return _lib.float_array([v for r in rows for v in r])
+
+
 def _coefficients(coefficients, steps):
-    rows = list(coefficients)
+    rows = tuple(coefficients)
     if rows and not hasattr(rows[0], '__len__'):
-        rows = [rows] * steps
+        rows = (rows,) * steps
+    else:
+        rows = tuple(tuple(r) for r in rows)
     if len(rows) != steps or any(len(r) != 3 for r in rows):
         raise ValueError('coefficients must be three numbers, or three for '
                          'each of the %d steps' % steps)
-    return _lib.float_array([v for r in rows for v in r])
+    return _coefficient_array(rows)
 
 
 def orthogonalize(xs, outs=None, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7,
@@ -1061,25 +1069,27 @@ def orthogonalize(xs, outs=None, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7,
     ``params`` (of the same types)
     param = (1 - lr * decay) * param - lr * scale * X in the last product's
     epilogue; only ``outs`` that are given are then written."""
-    if isinstance(xs, torch.Tensor):
-        got = orthogonalize([xs], None if outs is None else [outs], steps,
-                            coefficients, eps, [scale],
-                            None if params is None else [params], lr, decay)
-        return got[0]
+    single = isinstance(xs, torch.Tensor)
+    if single:
+        xs, scale = [xs], [scale]
+        outs = None if outs is None else [outs]
+        params = None if params is None else [params]
     xs = list(xs)
     count = len(xs)
     scales = list(scale) if hasattr(scale, '__len__') else [scale] * count
     outs = [None] * count if outs is None else list(outs)
-    weights = [None] * count if params is None else list(params)
-    if not len(scales) == len(outs) == len(weights) == count:
-        raise ValueError('%d matrices, %d outputs, %d scales, %d weights' % (
-            count, len(outs), len(scales), len(weights)))
+    if not len(scales) == len(outs) == count or \
+            (params is not None and len(params) != count):
+        raise ValueError('%d matrices, %d outputs, %d scales, %s weights' % (
+            count, len(outs), len(scales),
+            'no' if params is None else len(params)))
     if not 1 <= steps <= 64:
         raise ValueError('steps must be 1 to 64, got %d' % steps)
     coef = _coefficients(coefficients, steps)
     if not count:
         return outs
-    device = xs[0].device
+    index = xs[0].get_device()
+    weights = [None] * count if params is None else list(params)
     groups = {}
     for i, (x, out, w) in enumerate(zip(xs, outs, weights)):
         _chk_rows(x, 'x')
@@ -1089,28 +1099,33 @@ def orthogonalize(xs, outs=None, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7,
             if t is not None:
                 _chk_rows(t, name, (x.dtype,))
                 _chk_shape(t, x.shape, name)
-        _chk_place(device.index, ('x', x), ('out', out), ('param', w))
+                _chk_place(index, (name, t))
+        _chk_place(index, ('x', x))
         groups.setdefault(x.dtype, []).append(i)
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return orthogonalize(xs, outs, steps, coefficients, eps, scales,
-                                 params, lr, decay)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            got = orthogonalize(xs, outs, steps, coefficients, eps, scales,
+                                params, lr, decay)
+        return got[0] if single else got
     lib = _lib.load()
+    stream = _raw_stream(index)
     for dtype, idx in groups.items():
         part = [xs[i] for i in idx]
-        rows = _lib.int_array([x.shape[0] for x in part])
-        cols = _lib.int_array([x.numel() // x.shape[0] for x in part])
+        n = len(idx)
+        rows = (ctypes.c_int * n)(*[x.shape[0] for x in part])
+        cols = (ctypes.c_int * n)(*[x.numel() // x.shape[0] for x in part])
         for i in idx:
             if outs[i] is None and weights[i] is None:
                 outs[i] = torch.empty_like(xs[i])
-        ws = _scratch(lib.kfac_orthogonalize_workspace_bytes(
-            len(idx), rows, cols), device)
+        nbytes, ws = lib.kfac_orthogonalize_workspace_bytes(n, rows, cols), None
+        if nbytes:
+            ws = part[0].new_empty(nbytes, dtype=torch.uint8)
         _lib.check(lib.kfac_orthogonalize(
-            WIRE_DTYPES[dtype], len(idx), rows, cols,
+            WIRE_DTYPES[dtype], n, rows, cols,
             _lib.ptr_array([x.data_ptr() for x in part]),
             _lib.ptr_array([_p(outs[i]) for i in idx]),
+            None if params is None else
             _lib.ptr_array([_p(weights[i]) for i in idx]),
-            _lib.float_array([scales[i] for i in idx]), steps, coef, eps, lr,
-            decay, ws.data_ptr(), ws.numel(), _stream()),
-            'kfac_orthogonalize')
-    return outs
+            (ctypes.c_float * n)(*[scales[i] for i in idx]), steps, coef, eps,
+            lr, decay, _p(ws), nbytes, stream), 'kfac_orthogonalize')
+    return outs[0] if single else outs

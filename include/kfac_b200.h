@@ -556,7 +556,8 @@ int kfac_token_counts(const void* ids, int id_bytes, int64_t n, int64_t vocab,
  * fp32 products carry 22 bits of their operands; for 16-bit matrices A and the
  * polynomial carry 11.  An X with entries of 8 and more, or values that are
  * not finite, give NaN.  Pointer, size and coefficient arrays are host arrays
- * read during the call. */
+ * read during the call.  (Matrices of up to 128 and 256 a side, if all are,
+ * take one launch and no workspace.) */
 size_t kfac_orthogonalize_workspace_bytes(int count, const int* rows,
                                           const int* cols);
 int kfac_orthogonalize(int dtype, int count, const int* rows, const int* cols,

@@ -100,7 +100,8 @@ def test_orthogonalize_calls_are_checked(lib):
                 dict(out=[None], param=[None]), dict(count=-1)):
         assert ortho(lib, **bad) == 1, bad
         assert 'orthogonalize' in message(lib)
-    assert ortho(lib, nbytes=64) == 3 and ortho(lib, ws=None) == 3
+    big = dict(rows=[300], cols=[200])
+    assert ortho(lib, nbytes=64, **big) == 3 and ortho(lib, ws=None, **big) == 3
     assert ortho(lib, rows=[], cols=[], x=[], out=[], scale=[]) == 0
 
 
@@ -113,12 +114,16 @@ def test_workspace_of_an_orthogonalisation(lib):
         return lib.kfac_orthogonalize_workspace_bytes(
             len(shapes), _lib.int_array([s[0] for s in shapes]),
             _lib.int_array([s[1] for s in shapes]))
-    for r, c in ((1, 1), (64, 147), (1000, 24), (4096, 4096)):
+    for r, c in ((129, 130), (64, 257), (1000, 24), (4096, 4096)):
         small = min(r, c)
         least = 4 * (2 * r * c + 2 * small * small)
         assert least <= need((r, c)) <= \
             least + 4 * (2 * r * 8 + 2 * small * 8) + 8192
-    assert need((64, 64), (300, 20)) >= need((64, 64)) + need((300, 20)) - 512
+    assert need((300, 300), (300, 20)) >= \
+        need((300, 300)) + need((300, 20)) - 512
+    # small ones stay in shared memory, unless they ride along with others
+    assert need((1, 1), (64, 147), (256, 128)) == 0
+    assert need((64, 147), (300, 300)) > need((300, 300)) + 8 * 64 * 147
     assert need() == 0 and need((0, 4)) == 0
 
 

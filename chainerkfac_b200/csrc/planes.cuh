@@ -727,12 +727,13 @@ void plane_number_tiles(PlaneLaunch<N>& l) {
 
 // How many pairs share a tile: as many as a count of cycles comes out least for, with
 // `room[i]` clusters of 2^i pairs on the GPU at a time.  A k-block takes an MMA of 128
-// cycles for each 16 k and product of terms; a tile's start and end 6000 (beside the
-// next one's MMAs 2000), 18000 with a shared sum: the parts go through distributed
-// shared memory at 20 bytes a cycle and SM.  512 x 4608, whose X X^T has three tiles of
-// 72 k-blocks: five steps 342 us with eight pairs a tile, 373 with four; 2048 x 2048,
-// whose 36 tiles of 32 k-blocks do not all find room in pairs of pairs (33 do): 700 us
-// with one, 788 with two.
+// cycles for each 16 k and product of terms; a tile's start and end 11000 (beside the
+// next one's MMAs 2000), with a shared sum 8000 and 500 for each pair: its parts go
+// through distributed shared memory at 20 bytes a cycle and SM, but every pair has a
+// part of the epilogue only.  Five steps of 512 x 512, with three tiles: 220 us, 313
+// with 18000 for a shared sum and 6000 without; one matrix of each kind of ResNet-50
+// 522 us and 576.  2048 x 2048, whose 36 tiles do not all find room in pairs of pairs
+// (33 do): 690 us with one pair a tile, 900 with two.
 template <int N>
 int plane_split(const PlaneLaunch<N>& l, const int* room) {
   const double cycles = (l.terms - 1) * 4 * 132.0;
@@ -744,7 +745,7 @@ int plane_split(const PlaneLaunch<N>& l, const int* room) {
     for (int k = 0; k < l.n; ++k) {
       const int end = k + 1 < l.n ? l.p[k + 1].f.tile_begin : l.tiles;
       const int kb = (l.p[k].f.K + PL_BK - 1) / PL_BK;
-      const double one = (kb + s - 1) / s * cycles + (s > 1 ? 18000 : 2000);
+      const double one = (kb + s - 1) / s * cycles + (s > 1 ? 8000 + 500 * s : 2000);
       longest = std::max(longest, one);
       sum += one * (end - l.p[k].f.tile_begin);
     }
@@ -753,7 +754,7 @@ int plane_split(const PlaneLaunch<N>& l, const int* room) {
     const double time =
         std::max(longest, l.n == 1 ? sum / l.tiles * std::ceil(waves)
                                    : sum / l.tiles * waves + longest / 2) +
-        (s > 1 ? 0 : 4000);
+        (s > 1 ? 0 : 9000);
     if (s == 1 || time < best) {
       best = time;
       split = s;

@@ -329,12 +329,13 @@ int norm_blocks_of(long long count) {
       1, std::min<long long>(kNormBlocksMax, (count + kNormChunk - 1) / kNormChunk));
 }
 
-// Whether every matrix is one that a block orthogonalises by itself.  Beside larger
-// ones they ride along in the products' launches, which take no longer for them.
+// Whether every matrix is one that a block or a cluster orthogonalises by itself.
+// Beside larger ones they ride along in the products' launches, which take no longer
+// for them.
 bool all_small(int count, const int* rows, const int* cols) {
   for (int i = 0; i < count; ++i)
     if (std::min(rows[i], cols[i]) > kSmallShort ||
-        std::max(rows[i], cols[i]) > kSmallLong)
+        std::max(rows[i], cols[i]) > kSmallClusterLong)
       return false;
   return true;
 }

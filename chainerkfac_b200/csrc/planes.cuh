@@ -463,6 +463,8 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
     }
     __syncwarp();
   } else if (warp == 1) {
+    // (not before there is something to multiply: the waits are bounded)
+    wait_for_launch_before();
     if (side == 0 && elect_one()) {
       const unsigned short both = (unsigned short)(3u << first);
       int it = 0, seg = 0;

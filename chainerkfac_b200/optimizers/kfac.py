@@ -1267,10 +1267,12 @@ class DistributedKFAC(KFAC):
 def check_embeddings(fblocks):
     """An embedding's weight that another block updates too (an output layer
     that shares it) would be updated twice."""
+    if not any(isinstance(fb, FB.FisherBlockEmbedID) for fb in fblocks):
+        return
     owner = {}
     for fb in fblocks:
         for param in fb.link.params():
-            other = owner.setdefault(id(param._p), fb)
+            other = owner.setdefault(id(getattr(param, '_p', param)), fb)
             if other is not fb and (
                     isinstance(fb, FB.FisherBlockEmbedID) or
                     isinstance(other, FB.FisherBlockEmbedID)):

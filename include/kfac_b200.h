@@ -553,11 +553,11 @@ int kfac_token_counts(const void* ids, int id_bytes, int64_t n, int64_t vocab,
  * out[i] = scale[i] * X, and with a weight, param[i] of the same type,
  *     param = (1 - lr * decay) * param - lr * scale * X.
  * Either may be NULL, as arrays or element by element; out[i] may be x[i].
- * fp32 products carry 22 bits of their operands; for 16-bit matrices A and the
- * polynomial carry 11.  An X with entries of 8 and more, or values that are
+ * fp32 products carry 22 bits of their operands; for 16-bit matrices whose
+ * sides are both over 128, A and the polynomial carry 11.  An X with entries of 8 and more, or values that are
  * not finite, give NaN.  Pointer, size and coefficient arrays are host arrays
- * read during the call.  (Matrices of up to 128 and 256 a side, if all are,
- * take one launch and no workspace.) */
+ * read during the call.  (Matrices with one side of up to 128 and the
+ * other of up to 16 x 192 take one launch and no workspace, if all are.) */
 size_t kfac_orthogonalize_workspace_bytes(int count, const int* rows,
                                           const int* cols);
 int kfac_orthogonalize(int dtype, int count, const int* rows, const int* cols,

@@ -6,9 +6,10 @@ products deep, and an error of X, relative to its largest singular value, grows
 with the smallest ones by up to |a|^5 = 485 while it is spread over all of the
 result's sqrt(min side) of norm: 485 * 2^-22 = 1.2e-4 / sqrt(min side) in the
 worst case, 2e-5 being for min side >= 33 and twice that below.  16 bits: the
-result is rounded to eps / 2 and A and B to 2^-12 of entries of up to |b| = 4.8
-times order one in each step, of which the last two steps' are not damped:
-2 * 4.8 * 2^-12 = 2.4e-3 and eps / 2.
+result is rounded to eps / 2, and A and B to 2^-11 of their entries at most and
+2^-12 in the mean, where these are of order one and up to |b| = 4.8 times that;
+the last two steps' roundings are not damped: 2 * 4.8 * 2^-12 = 2.4e-3 and
+eps / 2.  (Small matrices round neither so far.)
 """
 
 import pytest
@@ -63,7 +64,10 @@ SHAPES = [(1, 1), (1, 9), (7, 1), (2, 3), (16, 16), (31, 200), (64, 147),
           (513, 512), (64, 1500), (1500, 200), (700, 1100),
           # what a block does by itself, turned and not, up to its sides
           (147, 64), (256, 128), (128, 256), (256, 33), (33, 255), (257, 128),
-          (128, 257), (129, 129), (48, 49), (90, 17)]
+          (128, 257), (129, 129), (48, 49), (90, 17),
+          # and the blocks of a cluster, from two to sixteen
+          (100, 384), (385, 33), (64, 576), (769, 128), (128, 1152), (1, 1537),
+          (2999, 65), (128, 3000), (127, 3100)]
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16,
@@ -107,6 +111,26 @@ def test_many_matrices_at_once(count):
         check(y.float() / s, x)
         # (alone a long sum may be cut elsewhere: near, not the same bits)
         assert torch.equal(y, z)
+
+
+def test_matrices_of_a_cluster_in_one_launch(dtype=torch.float32):
+    """Short ones beside long ones: some blocks of their clusters have no
+    columns."""
+    from chainerkfac_b200 import ops
+    g = gen(12)
+    xs = [torch.randn(s, device='cuda', generator=g).to(dtype) for s in
+          ((3, 2), (128, 2000), (1500, 40), (33, 33), (5, 900), (257, 128))]
+    got = ops.orthogonalize(xs)
+    again = ops.orthogonalize(xs)
+    for x, y, z in zip(xs, got, again):
+        check(y, x)
+        assert torch.equal(y, z)
+    # values that are not finite stay in their matrix
+    xs[1][7, 1999] = float('inf')
+    bad = ops.orthogonalize(xs)
+    assert bad[1].isnan().all()
+    for k in (0, 2, 3, 4, 5):
+        assert torch.equal(bad[k], got[k])
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])

@@ -41,28 +41,38 @@ struct EmbedStep {
   int* index;                      // their tokens
   int* row_exp;                    // of a row of `rows`
   int* col_exp;                    // of a row (and column) of G
-  bool vec;                        // rows of 16-byte words
+  bool vec;                        // all rows begin at 16 bytes
+  bool even;                       // kf, weights and velocities lie alike within 16 bytes
 };
 
+// A row of floats as up to three in front, words of 16 bytes, and up to three behind.
+struct RowWords {
+  int head, words, tail;
+};
+__device__ __forceinline__ RowWords row_words(const float* x, int width) {
+  RowWords w;
+  w.head = min((int)((-reinterpret_cast<uintptr_t>(x) & 15) >> 2), width);
+  w.words = (width - w.head) >> 2;
+  w.tail = width - w.head - 4 * w.words;
+  return w;
+}
+
 // Exponent of a row's largest value, by a warp; kNoExp: zeros.
-__device__ __forceinline__ int row_top(const float* x, int width, bool vec, int lane) {
+__device__ __forceinline__ int row_top(const float* x, int width, int lane) {
+  const RowWords w = row_words(x, width);
   int top = kNoExp;
-  if (vec) {
-    const float4* x4 = reinterpret_cast<const float4*>(x);
-    const int n = width >> 2;
+  if (lane < w.head) top = exp_of(x[lane]);
+  if (lane < w.tail) top = max(top, exp_of(x[w.head + 4 * w.words + lane]));
+  const float4* const x4 = reinterpret_cast<const float4*>(x + w.head);
 #pragma unroll 1
-    for (int k0 = lane; k0 < n; k0 += 256) {
-      float4 y[8];
+  for (int k0 = lane; k0 < w.words; k0 += 256) {
+    float4 y[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) y[u] = x4[min(k0 + 32 * u, n - 1)];
+    for (int u = 0; u < 8; ++u) y[u] = x4[min(k0 + 32 * u, w.words - 1)];
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        top = max(top, max(max(exp_of(y[u].x), exp_of(y[u].y)),
-                           max(exp_of(y[u].z), exp_of(y[u].w))));
-    }
-  } else {
-#pragma unroll 8
-    for (int k = lane; k < width; k += 32) top = max(top, exp_of(x[k]));
+    for (int u = 0; u < 8; ++u)
+      top = max(top, max(max(exp_of(y[u].x), exp_of(y[u].y)),
+                         max(exp_of(y[u].z), exp_of(y[u].w))));
   }
   return __reduce_max_sync(0xffffffffu, top);
 }
@@ -89,43 +99,58 @@ __device__ __forceinline__ void pack_planes(const float* x, int width, bool vec,
   }
 }
 
-// The update of a row without a gradient.
-__device__ __forceinline__ void rest_row(const EmbedStep& e, long long at, int lane) {
-  if (e.vec) {
-    const int n = e.width >> 2;
-#pragma unroll 1
-    for (int k0 = lane; k0 < n; k0 += 128) {
-      float4 v[4], p[4];
-      if (e.param != nullptr) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int k = min(k0 + 32 * u, n - 1);
-          v[u] = reinterpret_cast<const float4*>(e.mom + at)[k];
-          p[u] = reinterpret_cast<const float4*>(e.param + at)[k];
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int k = k0 + 32 * u;
-        if (k >= n) break;
-        reinterpret_cast<float4*>(e.kf + at)[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (e.param == nullptr) continue;
-        v[u].x *= e.momentum; v[u].y *= e.momentum;
-        v[u].z *= e.momentum; v[u].w *= e.momentum;
-        reinterpret_cast<float4*>(e.mom + at)[k] = v[u];
-        p[u].x += v[u].x; p[u].y += v[u].y; p[u].z += v[u].z; p[u].w += v[u].w;
-        reinterpret_cast<float4*>(e.param + at)[k] = p[u];
-      }
-    }
+// The update of a row: with its kf (GRADIENT), or without a gradient, kf = 0.
+template <bool GRADIENT>
+__device__ __forceinline__ void update_row(const EmbedStep& e, long long at, int lane) {
+  float* const kf = e.kf + at;
+  float* const mom = e.param != nullptr ? e.mom + at : nullptr;
+  float* const param = e.param != nullptr ? e.param + at : nullptr;
+  auto one = [&](int k) {
+    if (!GRADIENT) kf[k] = 0.f;
+    if (param == nullptr) return;
+    const float v = e.momentum * mom[k] - (GRADIENT ? e.lr * kf[k] : 0.f);
+    mom[k] = v;
+    param[k] += v;
+  };
+  if (!e.even) {
+#pragma unroll 4
+    for (int k = lane; k < e.width; k += 32) one(k);
     return;
   }
-#pragma unroll 4
-  for (int k = lane; k < e.width; k += 32) {
-    e.kf[at + k] = 0.f;
-    if (e.param == nullptr) continue;
-    const float v = e.momentum * e.mom[at + k];
-    e.mom[at + k] = v;
-    e.param[at + k] += v;
+  const RowWords w = row_words(kf, e.width);
+  if (lane < w.head) one(lane);
+  if (lane < w.tail) one(w.head + 4 * w.words + lane);
+  float4* const kf4 = reinterpret_cast<float4*>(kf + w.head);
+  float4* const mom4 = reinterpret_cast<float4*>(mom + w.head);
+  float4* const param4 = reinterpret_cast<float4*>(param + w.head);
+#pragma unroll 1
+  for (int k0 = lane; k0 < w.words; k0 += 128) {
+    float4 x[4], v[4], p[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = min(k0 + 32 * u, w.words - 1);
+      if (GRADIENT) x[u] = kf4[k];
+      if (param == nullptr) continue;
+      v[u] = mom4[k];
+      p[u] = param4[k];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = k0 + 32 * u;
+      if (k >= w.words) break;
+      if (!GRADIENT) kf4[k] = x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (param == nullptr) continue;
+      v[u].x = e.momentum * v[u].x - e.lr * x[u].x;
+      v[u].y = e.momentum * v[u].y - e.lr * x[u].y;
+      v[u].z = e.momentum * v[u].z - e.lr * x[u].z;
+      v[u].w = e.momentum * v[u].w - e.lr * x[u].w;
+      mom4[k] = v[u];
+      p[u].x += v[u].x;
+      p[u].y += v[u].y;
+      p[u].z += v[u].z;
+      p[u].w += v[u].w;
+      param4[k] = p[u];
+    }
   }
 }
 
@@ -140,9 +165,9 @@ embed_rows_kernel(const __grid_constant__ EmbedStep e) {
     const bool of_g = i < e.width;
     const long long row = of_g ? i : i - e.width;
     const float* x = (of_g ? e.G : e.grad) + row * e.width;
-    const int top = row_top(x, e.width, e.vec, lane);
+    const int top = row_top(x, e.width, lane);
     if (top == kNoExp && !of_g) {
-      rest_row(e, row * e.width, lane);
+      update_row<false>(e, row * e.width, lane);
       continue;
     }
     const int s = top == kNoExp ? 0 : kTopExp - top;
@@ -188,46 +213,43 @@ struct EpiEmbed {
     pl_put_floats(piece, v, lane);
     __syncwarp();
     const int rows = min(32, g.M - t.r0);
-    if (e.vec) {
+    // Two factors, of the column and of the row, where neither they nor what is
+    // between them can leave the range; else exponents added up for every value.
+    const int c1 = t.c0 + lane, ce1 = c1 < width ? e.col_exp[c1] : 0;
+    const bool near = abs(re) <= 60 && inv >= 1e-18f && inv <= 1e18f && abs(ce1) <= 60;
+    const bool fast = __all_sync(0xffffffffu, near);
+    const float row_f = fast ? scale_exp(inv, re) : inv;
+    const float col_f = scale_exp(1.f, ce1);
+    if (e.vec && fast) {
       const int c = t.c0 + 4 * (lane & 7);
-      const bool live = c < width;
-      // (the array's end is padded to whole words)
-      const int4 ce = live ? *reinterpret_cast<const int4*>(e.col_exp + c)
-                           : make_int4(0, 0, 0, 0);
-      // Two factors, of the column and of the row, where neither they nor what is
-      // between them can leave the range; else exponents added up for every value.
-      const bool near = abs(re) <= 60 && inv >= 1e-18f && inv <= 1e18f &&
-                        max(max(abs(ce.x), abs(ce.y)), max(abs(ce.z), abs(ce.w))) <= 60;
-      if (__all_sync(0xffffffffu, near)) {
-        const float row_f = scale_exp(inv, re);
-        const float4 col_f =
-            make_float4(scale_exp(1.f, ce.x), scale_exp(1.f, ce.y),
-                        scale_exp(1.f, ce.z), scale_exp(1.f, ce.w));
+      float4 f4;
+      f4.x = __shfl_sync(0xffffffffu, col_f, 4 * (lane & 7));
+      f4.y = __shfl_sync(0xffffffffu, col_f, 4 * (lane & 7) + 1);
+      f4.z = __shfl_sync(0xffffffffu, col_f, 4 * (lane & 7) + 2);
+      f4.w = __shfl_sync(0xffffffffu, col_f, 4 * (lane & 7) + 3);
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const int row = i + (lane >> 3);
-          const float f = __shfl_sync(0xffffffffu, row_f, row);
-          const int to = __shfl_sync(0xffffffffu, token, row);
-          float4 x = pl_word(piece, row, lane & 7);
-          x.x *= col_f.x * f;
-          x.y *= col_f.y * f;
-          x.z *= col_f.z * f;
-          x.w *= col_f.w * f;
-          if (live && row < rows)
-            *reinterpret_cast<float4*>(e.kf + (long long)to * width + c) = x;
-        }
-        return;
+      for (int i = 0; i < 32; i += 4) {
+        const int row = i + (lane >> 3);
+        const float f = __shfl_sync(0xffffffffu, row_f, row);
+        const int to = __shfl_sync(0xffffffffu, token, row);
+        float4 x = pl_word(piece, row, lane & 7);
+        x.x *= f4.x * f;
+        x.y *= f4.y * f;
+        x.z *= f4.z * f;
+        x.w *= f4.w * f;
+        if (c < width && row < rows)
+          *reinterpret_cast<float4*>(e.kf + (long long)to * width + c) = x;
       }
+      return;
     }
-    const int c = t.c0 + lane;
-    const int ce = c < width ? e.col_exp[c] : 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int row = 0; row < rows; ++row) {
       const int to = __shfl_sync(0xffffffffu, token, row);
       const int n = __shfl_sync(0xffffffffu, re, row);
-      const float f = __shfl_sync(0xffffffffu, inv, row);
-      const float x = scale_exp(pl_float(piece, row, lane), n + ce) * f;
-      if (c < width) e.kf[(long long)to * width + c] = x;
+      const float f = __shfl_sync(0xffffffffu, row_f, row);
+      float x = pl_float(piece, row, lane);
+      x = fast ? x * (col_f * f) : scale_exp(x, n + ce1) * f;
+      if (c1 < width) e.kf[(long long)to * width + c1] = x;
     }
   }
 };
@@ -236,48 +258,10 @@ struct EpiEmbed {
 __global__ void __launch_bounds__(kThreads)
 embed_update_kernel(const __grid_constant__ EmbedStep e) {
   wait_for_launch_before();
-  const int lane = threadIdx.x & 31;
   const int rows = *reinterpret_cast<const volatile int*>(e.count);
   for (int r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < rows;
-       r += gridDim.x * kWarps) {
-    const long long at = (long long)e.index[r] * e.width;
-    if (e.vec) {
-      const int n = e.width >> 2;
-#pragma unroll 1
-      for (int k0 = lane; k0 < n; k0 += 128) {
-        float4 x[4], v[4], p[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int k = min(k0 + 32 * u, n - 1);
-          x[u] = reinterpret_cast<const float4*>(e.kf + at)[k];
-          v[u] = reinterpret_cast<const float4*>(e.mom + at)[k];
-          p[u] = reinterpret_cast<const float4*>(e.param + at)[k];
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int k = k0 + 32 * u;
-          if (k >= n) break;
-          v[u].x = e.momentum * v[u].x - e.lr * x[u].x;
-          v[u].y = e.momentum * v[u].y - e.lr * x[u].y;
-          v[u].z = e.momentum * v[u].z - e.lr * x[u].z;
-          v[u].w = e.momentum * v[u].w - e.lr * x[u].w;
-          reinterpret_cast<float4*>(e.mom + at)[k] = v[u];
-          p[u].x += v[u].x;
-          p[u].y += v[u].y;
-          p[u].z += v[u].z;
-          p[u].w += v[u].w;
-          reinterpret_cast<float4*>(e.param + at)[k] = p[u];
-        }
-      }
-      continue;
-    }
-#pragma unroll 4
-    for (int k = lane; k < e.width; k += 32) {
-      const float v = e.momentum * e.mom[at + k] - e.lr * e.kf[at + k];
-      e.mom[at + k] = v;
-      e.param[at + k] += v;
-    }
-  }
+       r += gridDim.x * kWarps)
+    update_row<true>(e, (long long)e.index[r] * e.width, threadIdx.x & 31);
 }
 
 long long parts_of(long long a, long long b) { return (a + b - 1) / b; }
@@ -374,6 +358,9 @@ extern "C" int kfac_precondition_embedding(int64_t vocab, int width, const float
           ((reinterpret_cast<uintptr_t>(G_inv) | reinterpret_cast<uintptr_t>(grad) |
             reinterpret_cast<uintptr_t>(kf) | reinterpret_cast<uintptr_t>(param) |
             reinterpret_cast<uintptr_t>(mom)) & 15) == 0;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(kf);
+  e.even = param == nullptr || (((at - reinterpret_cast<uintptr_t>(param)) |
+                                 (at - reinterpret_cast<uintptr_t>(mom))) & 15) == 0;
   lay_out(vocab, width, ws, &e);
   cudaStream_t st = (cudaStream_t)stream;
   KFAC_CUDA(cudaMemsetAsync(e.count, 0, sizeof(int), st));

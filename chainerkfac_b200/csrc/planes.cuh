@@ -596,10 +596,15 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int col = 128 * h + 4 * i, owner = col / width;
-            const unsigned to = cluster_addr(base, 2 * owner + side);
-            cluster_store(to + ((part * 4 + q) * groups + (col - owner * width) / 4) *
-                                   512 + lane * 16,
-                          v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            const unsigned at =
+                base + ((part * 4 + q) * groups + (col - owner * width) / 4) * 512 +
+                lane * 16;
+            if (owner == part)
+              sts128(at, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2],
+                                     v[4 * i + 3]));
+            else
+              cluster_store(cluster_addr(at, 2 * owner + side), v[4 * i], v[4 * i + 1],
+                            v[4 * i + 2], v[4 * i + 3]);
           }
         }
         cluster_sync();

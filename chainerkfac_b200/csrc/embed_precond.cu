@@ -379,7 +379,6 @@ extern "C" int kfac_precondition_embedding(int64_t vocab, int width, const float
   if ((rc = plane_map(&l.p[0].ma, e.rows, (int)vocab, width, false)) != KFAC_OK ||
       (rc = plane_map(&l.p[0].mb, e.g, width, width, false)) != KFAC_OK)
     return rc;
-  plane_number_tiles(l);
   l.rows = e.count;
   rc = plane_launch("embed products", l, EpiEmbed{e}, true, st);
   if (rc != KFAC_OK || param == nullptr) return rc;

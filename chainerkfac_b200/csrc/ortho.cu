@@ -496,11 +496,10 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
   }
   for (int k = 0; k < 2; ++k) {
     gram[k].n = apply[k].n = n;
-    plane_number_tiles(gram[k]);
-    plane_number_tiles(apply[k]);
+    gram[k].rows = apply[k].rows = nullptr;
   }
   poly.n = n;
-  plane_number_tiles(poly);
+  poly.rows = nullptr;
   for (int step = 0; step < c.steps; ++step) {
     const float* k = c.coefficients + 3 * step;
     const int from = step & 1;

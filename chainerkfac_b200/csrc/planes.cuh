@@ -5,12 +5,14 @@
 // accumulator of their own: 22 significant bits.
 //
 // Tiles of 256 x 256 by pairs of CTAs (cta_group::2: each holds 128 rows of A and of
-// C, and half of B's rows), k-blocks of 64: TMA lays both operands out as the MMAs
-// read them, whether k runs along the rows or down the columns of the planes, and
-// fills zeros past the edges, so any size goes without a copy.  In each CTA warp 0
-// issues the loads and, in the first of a pair, warp 1 the MMAs; eight warps take the
-// accumulators, which are there twice, out of tensor memory while the MMAs go on in
-// the other one.
+// C, and half of B's rows), or of 128 x 128 by one CTA where there are few of them,
+// k-blocks of 64: TMA lays both operands out as the MMAs read them, whether k runs
+// along the rows or down the columns of the planes, and fills zeros past the edges, so
+// any size goes without a copy.  In each CTA warp 0 issues the loads and, in the first
+// of a pair, warp 1 the MMAs; eight warps take the accumulators, which are there twice,
+// out of tensor memory while the MMAs go on in the other one.  An MMA of 128 columns
+// takes 150 cycles behind one on the same accumulator instead of 64, one of 256 its
+// 128: the small tiles have cross terms in an accumulator of their own.
 //
 // The tensor core adds with truncation, so a long sum comes out too small by what
 // its number of additions makes: a sum of two-term products is cut every PL_SEGMENT
@@ -19,7 +21,7 @@
 // small.
 //
 // Launches with fewer tiles than the GPU has room for share the sum of a tile among
-// up to eight pairs of a cluster, which hand each other their parts through
+// up to eight pairs (four CTAs) of a cluster, which hand each other their parts through
 // distributed shared memory, added in the order of k.
 //
 // Every barrier wait is bounded; a wait that runs out raises the status word.
@@ -39,7 +41,6 @@ namespace kfac {
 // Status word of the bounded waits, one in each source file that has products.
 static __device__ int g_plane_status = 0;
 
-constexpr int PL_TILE = 256;                 // tile sides
 constexpr int PL_ROWS = 128;                 // rows of a CTA's part of A, B and C
 constexpr int PL_BK = 64;                    // k of a stage: 128 bytes of fp16
 constexpr int PL_TERM = PL_ROWS * PL_BK * 2; // bytes of one term of such a part
@@ -49,14 +50,16 @@ constexpr int PL_STAGES_MAX = 6;
 // 0.9e-6 with one, 3.9 ms and 1.9e-6 with two, 3.7 ms and 3.7e-6 with four: of one, a
 // segment is in the tensor cores for less time than it takes to read.
 constexpr int PL_SEGMENT = 2;
-constexpr int PL_SPLIT_MAX = 8;              // pairs that share a tile
 constexpr int PL_EPI_WARPS = 8;
 constexpr int PL_THREADS = 32 * (4 + PL_EPI_WARPS);
 constexpr int PL_PIECE = 4096;               // bytes of a warp's staging
 constexpr int PL_SMEM =
     PL_STAGE_BYTES + PL_EPI_WARPS * PL_PIECE + 1024 /* control */ + 1024 /* align */;
 constexpr int PL_COLS = 512;                 // tensor memory: two accumulators
-static_assert(PL_ROWS * PL_TILE * 4 <= PL_STAGE_BYTES, "parts of a shared sum");
+// Cycles of an MMA of 128 columns, and what a small tile takes beside its MMAs with a
+// shared sum and without (plane_split).
+constexpr double PL_SMALL_MMA = 100, PL_SMALL_SHARE = 5000, PL_SMALL_END = 5000;
+static_assert(PL_ROWS * 256 * 4 <= PL_STAGE_BYTES, "parts of a shared sum");
 
 // A pair of planes.
 struct Planes {
@@ -92,7 +95,7 @@ struct PlaneLaunch {
   int n;
   int tiles;
   int terms;             // of both operands
-  int split;             // pairs of CTAs that share a tile
+  int split;             // CTAs, or pairs of them, that share a tile
   const int* rows;       // the rows of a launch's only problem, where the device counts
                          // them (M is then the most there can be); or null
 };
@@ -136,24 +139,31 @@ __device__ __forceinline__ void cluster_store(unsigned addr, float a, float b, f
                : "memory");
 }
 
-// D = f32, A = B = f16, M = N = 256 by two CTAs.
-__device__ __forceinline__ unsigned pair_desc(bool a_mn, bool b_mn) {
+// D = f32, A = B = f16, M = N = 128 by one CTA, 256 by two.
+template <int G>
+__device__ __forceinline__ unsigned pl_desc(bool a_mn, bool b_mn) {
   return (1u << 4) | ((unsigned)a_mn << 15) | ((unsigned)b_mn << 16) |
-         ((unsigned)(PL_TILE >> 3) << 17) | ((unsigned)(PL_TILE >> 4) << 24);
+         ((unsigned)(128 * G >> 3) << 17) | ((unsigned)(128 * G >> 4) << 24);
 }
-__device__ __forceinline__ void pair_mma(unsigned tmem_d, unsigned long long da,
-                                         unsigned long long db, unsigned idesc,
-                                         unsigned accumulate) {
+template <int G>
+__device__ __forceinline__ void pl_mma(unsigned tmem_d, unsigned long long da,
+                                       unsigned long long db, unsigned idesc,
+                                       unsigned accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::%5.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "n"(G)
       : "memory");
 }
 // Arrives at the barrier in both CTAs of the pair (`mask`) once the MMAs are done.
-__device__ __forceinline__ void pair_commit(unsigned long long* bar,
-                                            unsigned short mask) {
+template <int G>
+__device__ __forceinline__ void pl_commit(unsigned long long* bar,
+                                          unsigned short mask) {
+  if (G == 1) {
+    tc_commit(bar);
+    return;
+  }
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster."
       "multicast::cluster.b64 [%0], %1;"
@@ -161,8 +171,18 @@ __device__ __forceinline__ void pair_commit(unsigned long long* bar,
       : "memory");
 }
 
+// G: CTAs of a tile.  Of a pair both count at the first one's barrier.
+template <int G>
 __device__ __forceinline__ void pl_load(unsigned dst, const CUtensorMap* map, int x,
                                         int y, int z, unsigned bar) {
+  if (G == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::"
+        "complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+    return;
+  }
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::"
       "complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
@@ -172,14 +192,15 @@ __device__ __forceinline__ void pl_load(unsigned dst, const CUtensorMap* map, in
 
 // One term of an operand tile: rows r0.. of it, k-block kb.  Rows down the planes: a
 // box of 128 rows x 64 k; rows along the planes: two boxes of 64 k x 64 rows.
+template <int G>
 __device__ __forceinline__ void pl_load_term(unsigned dst, const CUtensorMap* map,
                                              int mn, int r0, int kb, int term,
                                              unsigned bar) {
   if (!mn) {
-    pl_load(dst, map, kb * PL_BK, r0, term, bar);
+    pl_load<G>(dst, map, kb * PL_BK, r0, term, bar);
   } else {
-    pl_load(dst, map, r0, kb * PL_BK, term, bar);
-    pl_load(dst + PL_TERM / 2, map, r0 + 64, kb * PL_BK, term, bar);
+    pl_load<G>(dst, map, r0, kb * PL_BK, term, bar);
+    pl_load<G>(dst + PL_TERM / 2, map, r0 + 64, kb * PL_BK, term, bar);
   }
 }
 
@@ -338,6 +359,7 @@ __device__ __forceinline__ const PlaneProblem& pl_problem(const PlaneLaunch<N>& 
   return l.p[f];
 }
 
+template <int G>
 __device__ __forceinline__ void pl_tile_at(const PlaneFields& g, int tile, int& m0,
                                            int& n0) {
   const int t = tile - g.tile_begin;
@@ -348,17 +370,21 @@ __device__ __forceinline__ void pl_tile_at(const PlaneFields& g, int tile, int& 
     bi = t / g.tiles_n;
     bj = t - bi * g.tiles_n;
   }
-  m0 = bi * PL_TILE;
-  n0 = bj * PL_TILE;
+  m0 = bi * 128 * G;
+  n0 = bj * 128 * G;
 }
 
 // Epi: the epilogue's type.  epi.begin(problem, tile) is called for a warp's rows and
 // its first columns before the sums are there; epi.store(problem, tile, v, mirror,
 // what begin gave) takes the sums of a PlaneTile, unscaled.
-template <int N, typename Epi>
+// G: CTAs of a tile.
+template <int N, typename Epi, int G>
 __global__ void __launch_bounds__(PL_THREADS, 1)
 plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
              const __grid_constant__ Epi epi) {
+  constexpr int TILE = 128 * G;            // sides
+  constexpr int COLS = TILE / 2;           // columns of an epilogue's warp
+  constexpr int BUFFER = PL_COLS / 2;      // tensor memory of an accumulator
   int* const status = &g_plane_status;
   extern __shared__ unsigned char pl_smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
@@ -369,11 +395,11 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int stage_bytes = l.terms * PL_TERM;
   const int stages = PL_STAGE_BYTES / stage_bytes;
-  const bool cut = l.terms == 4;
+  const bool cut = l.terms == 4, cross = G == 1 && l.terms > 2;
   const int S = l.split;
-  const unsigned rank = cluster_rank(), first = rank & ~1u, side = rank & 1u;
-  const int part = (int)(rank >> 1);               // of a shared sum
-  const int tile0 = blockIdx.x / (2 * S), step = gridDim.x / (2 * S);
+  const unsigned rank = cluster_rank(), side = rank % G, first = rank - side;
+  const int part = (int)(rank / G);                // of a shared sum
+  const int tile0 = blockIdx.x / (G * S), step = gridDim.x / (G * S);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -383,7 +409,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
       }
       for (int b = 0; b < 2; ++b) {
         mbar_init(&ctl->accum[b], 1);
-        mbar_init(&ctl->drained[b], 2 * PL_EPI_WARPS);
+        mbar_init(&ctl->drained[b], G * PL_EPI_WARPS);
       }
       ctl->abort_flag = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -391,11 +417,12 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
     __syncwarp();
   } else if (warp == 1) {
     asm volatile(
-        "tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
-        ::"r"(smem_u32(&ctl->tmem_base)), "r"(PL_COLS)
+        "tcgen05.alloc.cta_group::%2.sync.aligned.shared::cta.b32 [%0], %1;"
+        ::"r"(smem_u32(&ctl->tmem_base)), "r"(PL_COLS), "n"(G)
         : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;"
-                 ::: "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::%0.sync.aligned;"
+                 ::"n"(G)
+                 : "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -415,7 +442,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
   if (l.rows != nullptr) {
     wait_for_launch_before();
     counted = *reinterpret_cast<const volatile int*>(l.rows);
-    tiles = (counted + PL_TILE - 1) / PL_TILE * l.p[0].f.tiles_n;
+    tiles = (counted + TILE - 1) / TILE * l.p[0].f.tiles_n;
   }
   if (warp == 0) {
     if (elect_one()) {
@@ -425,7 +452,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
         const PlaneProblem& p = pl_problem(l, tile);
         const PlaneFields g = p.f;
         int m0, n0, kb0, nkb;
-        pl_tile_at(g, tile, m0, n0);
+        pl_tile_at<G>(g, tile, m0, n0);
         range(g, kb0, nkb);
         const bool share = g.same && m0 == n0;
         const int ta = g.ta, tb = g.tb;
@@ -450,14 +477,14 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
           const unsigned bar = cluster_addr(smem_u32(&ctl->full[s]), first);
           if (side == 0)
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-                         ::"r"(smem_u32(&ctl->full[s])), "r"(2 * bytes)
+                         ::"r"(smem_u32(&ctl->full[s])), "r"(G * bytes)
                          : "memory");
           const unsigned st = smem_u32(smem + s * stage_bytes);
           for (int t = 0; t < ta; ++t)
-            pl_load_term(st + t * PL_TERM, &p.ma, g.a_mn, ra, kb, t, bar);
+            pl_load_term<G>(st + t * PL_TERM, &p.ma, g.a_mn, ra, kb, t, bar);
           if (share) continue;
           for (int t = 0; t < tb; ++t)
-            pl_load_term(st + (ta + t) * PL_TERM, &p.mb, g.b_mn, rb, kb, t, bar);
+            pl_load_term<G>(st + (ta + t) * PL_TERM, &p.mb, g.b_mn, rb, kb, t, bar);
         }
       }
     }
@@ -472,12 +499,12 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
       for (int tile = tile0; ok && tile < tiles; tile += step) {
         const PlaneFields g = pl_problem(l, tile).f;
         int m0, n0, kb0, nkb;
-        pl_tile_at(g, tile, m0, n0);
+        pl_tile_at<G>(g, tile, m0, n0);
         range(g, kb0, nkb);
         const bool share = g.same && m0 == n0;
         const int ta = g.ta, tb = g.tb;
         const bool amn = g.a_mn, bmn = g.b_mn;
-        const unsigned idesc = pair_desc(amn, bmn);
+        const unsigned idesc = pl_desc<G>(amn, bmn);
         // from 16 k to the next (16-byte units)
         const unsigned long long adv_a = (amn ? 2048 : 32) >> 4;
         const unsigned long long adv_b = (bmn ? 2048 : 32) >> 4;
@@ -488,7 +515,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
           const bool fresh = kb == 0 || (cut && kb % PL_SEGMENT == 0);
           if (fresh) {
             const int b = seg & 1;
-            d = tmem + b * PL_TILE;
+            d = tmem + b * BUFFER;
             if (seg >= 2 &&
                 !mbar_wait_status(&ctl->drained[b], ((seg >> 1) - 1) & 1,
                                   &ctl->abort_flag, status)) {
@@ -509,28 +536,39 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
           const unsigned long long b =
               bmn ? tc_smem_desc_mn(sb, PL_TERM / 2) : tc_smem_desc(sb);
           unsigned acc = !fresh;
-          if (tb == 2) {
+          if (G == 1) {
 #pragma unroll
             for (int kk = 0; kk < PL_BK / 16; ++kk) {
-              pair_mma(d, a + kk * adv_a, b + lo + kk * adv_b, idesc, acc);
+              const unsigned long long ak = a + kk * adv_a, bk = b + kk * adv_b;
+              if (tb == 2) pl_mma<G>(d + TILE, ak, bk + lo, idesc, acc);
+              pl_mma<G>(d, ak, bk, idesc, acc);
+              if (ta == 2) pl_mma<G>(d + TILE, ak + lo, bk, idesc, acc | (tb == 2));
+              acc = 1;
+            }
+          } else {
+            if (tb == 2) {
+#pragma unroll
+              for (int kk = 0; kk < PL_BK / 16; ++kk) {
+                pl_mma<G>(d, a + kk * adv_a, b + lo + kk * adv_b, idesc, acc);
+                acc = 1;
+              }
+            }
+            if (ta == 2) {
+#pragma unroll
+              for (int kk = 0; kk < PL_BK / 16; ++kk) {
+                pl_mma<G>(d, a + lo + kk * adv_a, b + kk * adv_b, idesc, acc);
+                acc = 1;
+              }
+            }
+#pragma unroll
+            for (int kk = 0; kk < PL_BK / 16; ++kk) {
+              pl_mma<G>(d, a + kk * adv_a, b + kk * adv_b, idesc, acc);
               acc = 1;
             }
           }
-          if (ta == 2) {
-#pragma unroll
-            for (int kk = 0; kk < PL_BK / 16; ++kk) {
-              pair_mma(d, a + lo + kk * adv_a, b + kk * adv_b, idesc, acc);
-              acc = 1;
-            }
-          }
-#pragma unroll
-          for (int kk = 0; kk < PL_BK / 16; ++kk) {
-            pair_mma(d, a + kk * adv_a, b + kk * adv_b, idesc, acc);
-            acc = 1;
-          }
-          pair_commit(&ctl->empty[s], both);
+          pl_commit<G>(&ctl->empty[s], both);
           if (kb + 1 == nkb || (cut && (kb + 1) % PL_SEGMENT == 0)) {
-            pair_commit(&ctl->accum[seg & 1], both);
+            pl_commit<G>(&ctl->accum[seg & 1], both);
             ++seg;
           }
         }
@@ -549,16 +587,16 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
       PlaneFields g = pl_problem(l, tile).f;
       if (l.rows != nullptr) g.M = counted;
       int m0, n0, kb0, nkb;
-      pl_tile_at(g, tile, m0, n0);
+      pl_tile_at<G>(g, tile, m0, n0);
       range(g, kb0, nkb);
       t.r0 = m0 + PL_ROWS * side + 32 * q;
       const bool mirror = g.lower && m0 != n0;
       const int nseg = cut ? (nkb + PL_SEGMENT - 1) / PL_SEGMENT : (nkb > 0 ? 1 : 0);
-      t.c0 = n0 + 128 * h;
+      t.c0 = n0 + COLS * h;
       const auto ahead = epi.begin(g, t);
-      float v[128];
+      float v[COLS];
 #pragma unroll
-      for (int i = 0; i < 128; ++i) v[i] = 0.f;
+      for (int i = 0; i < COLS; ++i) v[i] = 0.f;
 #pragma unroll 1
       for (int k = 0; k < nseg; ++k, ++seg) {
         const int b = seg & 1;
@@ -567,12 +605,21 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const unsigned at = tmem + ((unsigned)(32 * q) << 16) + b * PL_TILE + 128 * h;
+        const unsigned at = tmem + ((unsigned)(32 * q) << 16) + b * BUFFER + COLS * h;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < COLS / 32; ++u) {
           float x[16], y[16];
           tc_ld_16x32(at + 32 * u, x);
           tc_ld_16x32(at + (16u << 16) + 32 * u, y);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            v[32 * u + i] += x[i];
+            v[32 * u + 16 + i] += y[i];
+          }
+          if (!cross) continue;
+          tc_ld_16x32(at + TILE + 32 * u, x);
+          tc_ld_16x32(at + (16u << 16) + TILE + 32 * u, y);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -589,13 +636,13 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
         // A shared sum (the cluster's only tile): the pairs own a part of the columns
         // each, a multiple of the 32 that 32 registers hold.  Parts lie by pair, rows'
         // quarter, four registers, lane.
-        const int width = PL_TILE / S, groups = width / 4;
+        const int width = TILE / S, groups = width / 4;
         const unsigned base = smem_u32(smem);
         cluster_sync();                      // the MMAs have read all stages
         if (ok) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int col = 128 * h + 4 * i, owner = col / width;
+          for (int i = 0; i < COLS / 4; ++i) {
+            const int col = COLS * h + 4 * i, owner = col / width;
             const unsigned at =
                 base + ((part * 4 + q) * groups + (col - owner * width) / 4) * 512 +
                 lane * 16;
@@ -603,7 +650,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
               sts128(at, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2],
                                      v[4 * i + 3]));
             else
-              cluster_store(cluster_addr(at, 2 * owner + side), v[4 * i], v[4 * i + 1],
+              cluster_store(cluster_addr(at, G * owner + side), v[4 * i], v[4 * i + 1],
                             v[4 * i + 2], v[4 * i + 3]);
           }
         }
@@ -636,8 +683,8 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
       }
       if (!ok) break;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        t.c0 = n0 + 128 * h + 32 * u;
+      for (int u = 0; u < COLS / 32; ++u) {
+        t.c0 = n0 + COLS * h + 32 * u;
         float x[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) x[i] = v[32 * u + i];
@@ -653,7 +700,8 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
   __syncthreads();
   // (nobody leaves while the other may still arrive at its barriers)
   cluster_sync();
-  if (warp == 1) tc_release(tmem, PairColumns{PL_COLS}, ctl->abort_flag != 0);
+  using Columns = typename std::conditional<G == 2, PairColumns, unsigned>::type;
+  if (warp == 1) tc_release(tmem, Columns{PL_COLS}, ctl->abort_flag != 0);
 }
 
 // ----------------------------------------------------------------- host side
@@ -708,28 +756,28 @@ inline int plane_map(CUtensorMap* map, const Planes& o, int rows, int cols, bool
 // the 4 n others 1 / 4n, 2 / 4n .. 1: 6 n - 3.5 whole ones.  Errors of orthogonalised
 // 4096 x 4096 and 1024 x 4096 against fp64, with and without:
 // 1.9e-6 and 3.0e-6, 2.3e-6 and 4.0e-6 (fp32 products: 4.3e-6, 3.7e-6).
-inline float plane_gain(int terms, int K) {
+// (Small tiles have the cross terms elsewhere: 2 n + 0.5.)
+inline float plane_gain(int terms, int K, int G) {
   if (terms < 4) return 1.f;
   const int n = std::min((K + PL_BK - 1) / PL_BK, PL_SEGMENT);
-  return 1.f + (6 * n - 3.5f) * 0.72f * exp2f(-24);
+  return 1.f + (G == 2 ? 6 * n - 3.5f : 2 * n + 0.5f) * 0.72f * exp2f(-24);
 }
 
-// Numbers the tiles of l.p[0 .. l.n).
+// Numbers the tiles of l.p[0 .. l.n), of G blocks each.
 template <int N>
-void plane_number_tiles(PlaneLaunch<N>& l) {
+void plane_number_tiles(PlaneLaunch<N>& l, int G) {
   int total = 0;
+  const int side = 128 * G;
   for (int i = 0; i < l.n; ++i) {
     PlaneFields& g = l.p[i].f;
-    const int tm = (g.M + PL_TILE - 1) / PL_TILE, tn = (g.N + PL_TILE - 1) / PL_TILE;
+    const int tm = (g.M + side - 1) / side, tn = (g.N + side - 1) / side;
     g.tiles_n = tn;
     g.tile_begin = total;
     total += g.lower ? tm * (tm + 1) / 2 : tm * tn;
-    g.gain = plane_gain(g.ta + g.tb, g.K);
+    g.gain = plane_gain(g.ta + g.tb, g.K, G);
   }
   l.tiles = total;
   l.terms = l.n > 0 ? l.p[0].f.ta + l.p[0].f.tb : 0;
-  l.split = 1;
-  l.rows = nullptr;
 }
 
 // How many pairs share a tile: as many as a count of cycles comes out least for, with
@@ -741,18 +789,24 @@ void plane_number_tiles(PlaneLaunch<N>& l) {
 // with 18000 for a shared sum and 6000 without; one matrix of each kind of ResNet-50
 // 522 us and 576.  2048 x 2048, whose 36 tiles do not all find room in pairs of pairs
 // (33 do): 690 us with one pair a tile, 900 with two.
+struct PlaneShape {
+  int G, split;
+  double cycles;
+};
 template <int N>
-int plane_split(const PlaneLaunch<N>& l, const int* room) {
-  const double cycles = (l.terms - 1) * 4 * 132.0;
-  double best = 0;
-  int split = 1;
-  for (int i = 0, s = 1; s <= PL_SPLIT_MAX; ++i, s *= 2) {
+void plane_split(const PlaneLaunch<N>& l, int G, const int* room, PlaneShape& best) {
+  // of a k-block: MMAs of 256 columns, or of 128 in one or two accumulators
+  const double cycles = G == 2           ? (l.terms - 1) * 4 * 132.0
+                        : l.terms == 2 ? 4 * 150.0
+                                       : (l.terms - 1) * 4 * PL_SMALL_MMA;
+  for (int i = 0, s = 1; i < 4 && s <= (G == 2 ? 8 : 4); ++i, s *= 2) {
     if (room[i] <= 0) break;
+    const double more = s > 1 ? (G == 2 ? 8000 : PL_SMALL_SHARE) + 500 * s : 2000;
     double longest = 0, sum = 0;
     for (int k = 0; k < l.n; ++k) {
       const int end = k + 1 < l.n ? l.p[k + 1].f.tile_begin : l.tiles;
       const int kb = (l.p[k].f.K + PL_BK - 1) / PL_BK;
-      const double one = (kb + s - 1) / s * cycles + (s > 1 ? 8000 + 500 * s : 2000);
+      const double one = (kb + s - 1) / s * cycles + more;
       longest = std::max(longest, one);
       sum += one * (end - l.p[k].f.tile_begin);
     }
@@ -761,63 +815,90 @@ int plane_split(const PlaneLaunch<N>& l, const int* room) {
     const double time =
         std::max(longest, l.n == 1 ? sum / l.tiles * std::ceil(waves)
                                    : sum / l.tiles * waves + longest / 2) +
-        (s > 1 ? 0 : 9000);
-    if (s == 1 || time < best) {
-      best = time;
-      split = s;
-    }
+        (s > 1 ? 0 : G == 2 ? 9000 : PL_SMALL_END);
+    if (best.G == 0 || time < best.cycles) best = {G, s, time};
   }
-  return split;
+}
+
+// Clusters of G blocks times 1, 2, 4 and 8 that the device has room for.
+template <int N, typename Epi, int G>
+int plane_prepare(const char* name, int* room) {
+  KFAC_CUDA(cudaFuncSetAttribute(plane_kernel<N, Epi, G>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, PL_SMEM));
+  KFAC_CUDA(cudaFuncSetAttribute(plane_kernel<N, Epi, G>,
+                                 cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(PL_THREADS);
+  cfg.dynamicSmemBytes = PL_SMEM;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  for (int i = 3; i >= 0; --i) {
+    attr[0].val.clusterDim.x = G << i;
+    cfg.gridDim = dim3((G << i) * 64);
+    int n = 0;
+    KFAC_CUDA(cudaOccupancyMaxActiveClusters(&n, plane_kernel<N, Epi, G>, &cfg));
+    room[i] = n > 0 ? n : -1;
+  }
+  KFAC_REQUIRE(room[0] > 0, "%s: no room for a block", name);
+  return KFAC_OK;
 }
 
 template <int N, typename Epi>
 int plane_launch(const char* name, PlaneLaunch<N>& l, const Epi& epi, bool early,
                  cudaStream_t stream) {
-  if (l.tiles == 0) return KFAC_OK;
+  if (l.n == 0) return KFAC_OK;
   static std::mutex mu;
-  static int room[64][4];                      // 0: not asked yet
+  static int rooms[64][2][4];                  // by G; 0: not asked yet
   int dev = 0;
   KFAC_CUDA(cudaGetDevice(&dev));
   KFAC_REQUIRE(dev >= 0 && dev < 64, "device index %d unsupported", dev);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (rooms[dev][1][0] == 0) {
+      int room[2][4];
+      int rc = plane_prepare<N, Epi, 1>(name, room[0]);
+      if (rc == KFAC_OK) rc = plane_prepare<N, Epi, 2>(name, room[1]);
+      if (rc != KFAC_OK) return rc;
+      for (int k = 0; k < 8; ++k) rooms[dev][k / 4][k % 4] = room[k / 4][k % 4];
+    }
+  }
+  PlaneShape best = {0, 1, 0};
+  if (l.rows != nullptr) {
+    // (how many tiles there are is not known, and a cluster that shares one has one)
+    best.G = 2;
+  } else {
+    for (int G = 2; G >= 1; --G) {
+      plane_number_tiles(l, G);
+      plane_split(l, G, rooms[dev][G - 1], best);
+    }
+  }
+  plane_number_tiles(l, best.G);
+  l.split = best.split;
+  const int cluster = best.G * l.split;
+  const int clusters =
+      l.split > 1 ? l.tiles : std::min(l.tiles, rooms[dev][best.G - 1][0]);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster * clusters);
   cfg.blockDim = dim3(PL_THREADS);
   cfg.dynamicSmemBytes = PL_SMEM;
   cfg.stream = stream;
   cfg.attrs = attr;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (room[dev][0] == 0) {
-      KFAC_CUDA(cudaFuncSetAttribute(plane_kernel<N, Epi>,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     PL_SMEM));
-      KFAC_CUDA(cudaFuncSetAttribute(plane_kernel<N, Epi>,
-                                     cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-      for (int i = 3; i >= 0; --i) {
-        attr[0].val.clusterDim.x = 2 << i;
-        cfg.gridDim = dim3((2 << i) * 64);
-        cfg.numAttrs = 1;
-        int n = 0;
-        KFAC_CUDA(cudaOccupancyMaxActiveClusters(&n, plane_kernel<N, Epi>, &cfg));
-        room[dev][i] = n > 0 ? n : -1;
-      }
-      KFAC_REQUIRE(room[dev][0] > 0, "%s: no room for a pair of blocks", name);
-    }
-  }
-  // (a cluster that shares a tile has one, so the number has to be known)
-  l.split = l.rows != nullptr ? 1 : plane_split(l, room[dev]);
-  const int cluster = 2 * l.split;
-  const int clusters = l.split > 1 ? l.tiles : std::min(l.tiles, room[dev][0]);
-  attr[0].val.clusterDim.x = cluster;
-  cfg.gridDim = dim3(cluster * clusters);
   cfg.numAttrs = early ? 2 : 1;
-  KFAC_CUDA(cudaLaunchKernelEx(&cfg, plane_kernel<N, Epi>, l, epi));
+  if (best.G == 2)
+    KFAC_CUDA(cudaLaunchKernelEx(&cfg, plane_kernel<N, Epi, 2>, l, epi));
+  else
+    KFAC_CUDA(cudaLaunchKernelEx(&cfg, plane_kernel<N, Epi, 1>, l, epi));
   KFAC_LAUNCH_CHECK(name);
   return KFAC_OK;
 }

@@ -58,7 +58,7 @@ constexpr int PL_SMEM =
 constexpr int PL_COLS = 512;                 // tensor memory: two accumulators
 // Cycles of an MMA of 128 columns, and what a small tile takes beside its MMAs with a
 // shared sum and without (plane_split).
-constexpr double PL_SMALL_MMA = 100, PL_SMALL_SHARE = 5000, PL_SMALL_END = 5000;
+constexpr double PL_SMALL_MMA = 85, PL_SMALL_SHARE = 5000, PL_SMALL_END = 5000;
 static_assert(PL_ROWS * 256 * 4 <= PL_STAGE_BYTES, "parts of a shared sum");
 
 // A pair of planes.
@@ -780,15 +780,16 @@ void plane_number_tiles(PlaneLaunch<N>& l, int G) {
   l.terms = l.n > 0 ? l.p[0].f.ta + l.p[0].f.tb : 0;
 }
 
-// How many pairs share a tile: as many as a count of cycles comes out least for, with
-// `room[i]` clusters of 2^i pairs on the GPU at a time.  A k-block takes an MMA of 128
-// cycles for each 16 k and product of terms; a tile's start and end 11000 (beside the
-// next one's MMAs 2000), with a shared sum 8000 and 500 for each pair: its parts go
-// through distributed shared memory at 20 bytes a cycle and SM, but every pair has a
-// part of the epilogue only.  Five steps of 512 x 512, with three tiles: 220 us, 313
-// with 18000 for a shared sum and 6000 without; one matrix of each kind of ResNet-50
-// 522 us and 576.  2048 x 2048, whose 36 tiles do not all find room in pairs of pairs
-// (33 do): 690 us with one pair a tile, 900 with two.
+// Small tiles or large ones, and how many blocks or pairs share one: what a count of
+// cycles comes out least for, with `room[i]` clusters of 2^i of them on the GPU at a
+// time.  A k-block takes an MMA of 128 cycles (small tiles 85, or 150 behind each other)
+// for each 16 k and product of terms; a tile's start and end 11000 (small 7000; beside
+// the next one's MMAs 2000), with a shared sum 8000 (5000) and 500 for each that shares:
+// the parts go through distributed shared memory at 20 bytes a cycle and SM, but each
+// has a part of the epilogue only.  Five steps, us so, and with large tiles only: 256 x
+// 512 139 and 194, 512 x 512 155 and 215, 1000 x 1000 242 and 279, 512 x 4608 232 and
+// 293, one matrix of each kind of ResNet-50 464 and 520; with small tiles only 1024 x
+// 4096 412 (378 so), 2048 x 2048 625 (578).
 struct PlaneShape {
   int G, split;
   double cycles;
@@ -867,14 +868,12 @@ int plane_launch(const char* name, PlaneLaunch<N>& l, const Epi& epi, bool early
     }
   }
   PlaneShape best = {0, 1, 0};
-  if (l.rows != nullptr) {
-    // (how many tiles there are is not known, and a cluster that shares one has one)
-    best.G = 2;
-  } else {
-    for (int G = 2; G >= 1; --G) {
-      plane_number_tiles(l, G);
-      plane_split(l, G, rooms[dev][G - 1], best);
-    }
+  for (int G = 2; G >= 1; --G) {
+    // (where the device counts the rows, as if there were all; a cluster that shares a
+    // tile has one, so there a tile has its block or pair)
+    plane_number_tiles(l, G);
+    const int alone[4] = {rooms[dev][G - 1][0], 0, 0, 0};
+    plane_split(l, G, l.rows != nullptr ? alone : rooms[dev][G - 1], best);
   }
   plane_number_tiles(l, best.G);
   l.split = best.split;

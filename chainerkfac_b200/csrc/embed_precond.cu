@@ -213,14 +213,15 @@ struct EpiEmbed {
     pl_put_floats(piece, v, lane);
     __syncwarp();
     const int rows = min(32, g.M - t.r0);
-    // Two factors, of the column and of the row, where neither they nor what is
-    // between them can leave the range; else exponents added up for every value.
+    // Two factors, of the column and of the row, where neither they nor their product
+    // (2^-120 .. 2^120) can leave the range; else exponents added up for a value.  Which
+    // of them depends on its own row and column only, not on the rows beside it.
     const int c1 = t.c0 + lane, ce1 = c1 < width ? e.col_exp[c1] : 0;
-    const bool near = abs(re) <= 60 && inv >= 1e-18f && inv <= 1e18f && abs(ce1) <= 60;
-    const bool fast = __all_sync(0xffffffffu, near);
-    const float row_f = fast ? scale_exp(inv, re) : inv;
-    const float col_f = scale_exp(1.f, ce1);
-    if (e.vec && fast) {
+    const float row_f = scale_exp(inv, re), col_f = scale_exp(1.f, ce1);
+    const bool near_row = abs(re) <= 60 && row_f >= 1e-18f && row_f <= 1e18f;
+    const bool near_col = abs(ce1) <= 60;
+    const unsigned near_rows = __ballot_sync(0xffffffffu, near_row);
+    if (e.vec && near_rows == 0xffffffffu && __all_sync(0xffffffffu, near_col)) {
       const int c = t.c0 + 4 * (lane & 7);
       float4 f4;
       f4.x = __shfl_sync(0xffffffffu, col_f, 4 * (lane & 7));
@@ -247,8 +248,10 @@ struct EpiEmbed {
       const int to = __shfl_sync(0xffffffffu, token, row);
       const int n = __shfl_sync(0xffffffffu, re, row);
       const float f = __shfl_sync(0xffffffffu, row_f, row);
+      const float d = __shfl_sync(0xffffffffu, inv, row);
       float x = pl_float(piece, row, lane);
-      x = fast ? x * (col_f * f) : scale_exp(x, n + ce1) * f;
+      x = near_col && ((near_rows >> row) & 1) ? x * (col_f * f)
+                                               : scale_exp(x, n + ce1) * d;
       if (c1 < width) e.kf[(long long)to * width + c1] = x;
     }
   }

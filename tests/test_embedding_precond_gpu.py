@@ -113,6 +113,28 @@ def test_rows_of_any_size_and_not_finite():
         assert torch.equal(got[keep], base[keep])
 
 
+@pytest.mark.parametrize('width', [33, 96])
+def test_zeros_stay_beside_results_out_of_range(width):
+    """Factors of a row and of a column that fit, with a product that does not:
+    a zero stays a zero, whatever the rows next to it are like."""
+    from chainerkfac_b200 import ops
+    G_inv = torch.eye(width, device='cuda') * 2.0 ** 60
+    A = torch.zeros(64, device='cuda')
+    damping = torch.full((1,), 2.0 ** -55, device='cuda')
+    grad = torch.zeros((64, width), device='cuda')
+    grad[::2, 5] = 2.0 ** 60
+    grad[1::4, 7] = 2.0 ** -100
+    kf, bound = want_kf(G_inv, A, damping, grad)
+    got = ops.precondition_embedding(G_inv, A, damping, grad)
+    # (what makes up for truncation, at most (6 * 2 - 3.5) 0.72 2^-24 < 2^-21 of a
+    # value, is in the bound: finite values are not exact powers of two)
+    want = kf.float()
+    assert torch.equal(got.isinf(), want.isinf()) and int(got.isinf().sum()) == 32
+    assert torch.equal(got == 0, want == 0) and not got.isnan().any()
+    fine = want.isfinite()
+    assert bool(((got.double() - kf).abs() <= bound)[fine].all())
+
+
 def test_columns_of_different_sizes():
     """Features that never saw a gradient have large entries in G_inv."""
     from chainerkfac_b200 import ops

@@ -43,6 +43,16 @@ inline int fail(int code, const char* fmt, ...) {
     if (!(cond)) return ::kfac::fail(KFAC_ERR_INVALID, __VA_ARGS__);        \
   } while (0)
 
+// Whether two pieces of memory have bytes in common.
+inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a != nullptr && b != nullptr && a_bytes > 0 && b_bytes > 0 &&
+         x < y + b_bytes && y < x + a_bytes;
+}
+inline bool aligned_to(const void* p, size_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0;
+}
+
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Counter behind kfac_launch_count().

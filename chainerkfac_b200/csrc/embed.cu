@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <initializer_list>
 
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -691,6 +692,8 @@ int check_ids(const char* what, const void* ids, int id_bytes, int64_t n,
   KFAC_REQUIRE(vocab >= 1 && vocab < (1LL << 31) - 1,
                "%s: a vocabulary of %lld tokens", what, (long long)vocab);
   KFAC_REQUIRE(n == 0 || ids != nullptr, "%s: null pointer", what);
+  KFAC_REQUIRE(aligned_to(ids, id_bytes), "%s: tokens not aligned to %d bytes", what,
+               id_bytes);
   return KFAC_OK;
 }
 
@@ -698,7 +701,20 @@ int check_rows(const char* what, int dtype, int width) {
   KFAC_REQUIRE(dtype == KFAC_WIRE_F32 || dtype == KFAC_WIRE_F16 ||
                    dtype == KFAC_WIRE_BF16,
                "%s: unknown element type %d", what, dtype);
-  KFAC_REQUIRE(width >= 1, "%s: rows of %d values", what, width);
+  KFAC_REQUIRE(width >= 1 && width <= (1 << 28), "%s: rows of %d values (1 .. 2^28)",
+               what, width);
+  return KFAC_OK;
+}
+
+// Pieces of memory that a call reads, or writes besides.
+struct Piece {
+  const void* p;
+  size_t bytes;
+};
+int check_apart(const char* what, Piece out, std::initializer_list<Piece> others) {
+  for (const Piece& o : others)
+    KFAC_REQUIRE(!overlap(out.p, out.bytes, o.p, o.bytes),
+                 "%s: what is written overlaps another array", what);
   return KFAC_OK;
 }
 
@@ -877,6 +893,12 @@ extern "C" int kfac_embedding(int dtype, const void* weight, int64_t vocab,
   if (rc == KFAC_OK) rc = check_rows("embedding", dtype, width);
   if (rc != KFAC_OK || n == 0) return rc;
   KFAC_REQUIRE(weight != nullptr && out != nullptr, "embedding: null pointer");
+  const size_t size = type_size(dtype);
+  KFAC_REQUIRE(aligned_to(weight, size) && aligned_to(out, size),
+               "embedding: rows not aligned to their type");
+  rc = check_apart("embedding", {out, (size_t)n * width * size},
+                   {{weight, (size_t)vocab * width * size}, {ids, (size_t)n * id_bytes}});
+  if (rc != KFAC_OK) return rc;
   const Ids s = make_ids(ids, id_bytes, n, vocab, has_ignore, ignore);
   const int word = word_bytes(weight, out, width, dtype);
   cudaStream_t st = (cudaStream_t)stream;
@@ -897,7 +919,7 @@ extern "C" int kfac_token_order(const void* ids, int id_bytes, int64_t n,
                                 int64_t vocab, int has_ignore, int64_t ignore,
                                 int* keys, int* positions, void* workspace,
                                 size_t workspace_bytes, void* stream) {
-  const int rc = check_ids("token_order", ids, id_bytes, n, vocab);
+  int rc = check_ids("token_order", ids, id_bytes, n, vocab);
   if (rc != KFAC_OK || n == 0) return rc;
   KFAC_REQUIRE(keys != nullptr && positions != nullptr,
                "token_order: null pointer");
@@ -908,6 +930,15 @@ extern "C" int kfac_token_order(const void* ids, int id_bytes, int64_t n,
                 workspace == nullptr ? (size_t)0 : workspace_bytes, need);
   KFAC_REQUIRE(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
                "token_order: the workspace is not aligned to 4 bytes");
+  KFAC_REQUIRE(aligned_to(keys, 4) && aligned_to(positions, 4),
+               "token_order: keys or positions not aligned to 4 bytes");
+  const size_t bytes = (size_t)n * 4;
+  rc = check_apart("token_order", {keys, bytes},
+                   {{positions, bytes}, {ids, (size_t)n * id_bytes}, {workspace, need}});
+  if (rc == KFAC_OK)
+    rc = check_apart("token_order", {positions, bytes},
+                     {{ids, (size_t)n * id_bytes}, {workspace, need}});
+  if (rc != KFAC_OK) return rc;
   const Ids s = make_ids(ids, id_bytes, n, vocab, has_ignore, ignore);
   cudaStream_t st = (cudaStream_t)stream;
   if (n <= kClusterTokens) return sort_in_cluster(s, p, keys, positions, st);
@@ -966,6 +997,13 @@ extern "C" int kfac_embedding_grad(int dtype, const void* gy, int width,
                 workspace == nullptr ? (size_t)0 : workspace_bytes, need);
   KFAC_REQUIRE(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
                "embedding_grad: the workspace is not aligned to 16 bytes");
+  const size_t size = type_size(dtype), tokens = (size_t)n * 4;
+  KFAC_REQUIRE(aligned_to(gy, size) && aligned_to(out, size) && aligned_to(positions, 4),
+               "embedding_grad: arrays not aligned to their types");
+  rc = check_apart("embedding_grad", {out, (size_t)vocab * width * size},
+                   {{gy, (size_t)n * width * size}, {keys, tokens}, {positions, tokens},
+                    {workspace, need}});
+  if (rc != KFAC_OK) return rc;
   Grad g = {};
   g.keys = keys;
   g.perm = positions;
@@ -991,7 +1029,7 @@ extern "C" int kfac_token_counts(const void* ids, int id_bytes, int64_t n,
                                  float alpha, float beta, float* out, float* mean,
                                  void* workspace, size_t workspace_bytes,
                                  void* stream) {
-  const int rc = check_ids("token_counts", ids, id_bytes, n, vocab);
+  int rc = check_ids("token_counts", ids, id_bytes, n, vocab);
   if (rc != KFAC_OK) return rc;
   KFAC_REQUIRE(out != nullptr, "token_counts: null pointer");
   const size_t need = kfac_token_counts_workspace_bytes(vocab);
@@ -1000,6 +1038,14 @@ extern "C" int kfac_token_counts(const void* ids, int id_bytes, int64_t n,
                 workspace == nullptr ? (size_t)0 : workspace_bytes, need);
   KFAC_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
                "token_counts: the workspace is not aligned to 4 bytes");
+  KFAC_REQUIRE(aligned_to(out, 4) && aligned_to(mean, 4),
+               "token_counts: counts not aligned to 4 bytes");
+  const Piece tokens = {ids, (size_t)n * id_bytes}, scratch = {workspace, need};
+  rc = check_apart("token_counts", {out, (size_t)vocab * 4},
+                   {tokens, scratch, {mean, sizeof(float)}});
+  if (rc == KFAC_OK)
+    rc = check_apart("token_counts", {mean, sizeof(float)}, {tokens, scratch});
+  if (rc != KFAC_OK) return rc;
   int* counts = static_cast<int*>(workspace);
   cudaStream_t st = (cudaStream_t)stream;
   KFAC_CUDA(cudaMemsetAsync(counts, 0, need, st));

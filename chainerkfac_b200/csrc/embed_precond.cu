@@ -343,6 +343,29 @@ extern "C" int kfac_precondition_embedding(int64_t vocab, int width, const float
     return fail(KFAC_ERR_WORKSPACE,
                 "precondition_embedding: %zu bytes of workspace, %zu needed",
                 workspace == nullptr ? (size_t)0 : workspace_bytes, need);
+  // (kf may be where the gradient was: a row is read before its kf is there)
+  const size_t all = (size_t)vocab * width * sizeof(float);
+  struct Piece {
+    const void* p;
+    size_t bytes;
+    bool written;
+  };
+  const Piece pieces[] = {{kf, all, true},
+                          {param, all, true},
+                          {mom, all, true},
+                          {grad, all, false},
+                          {G_inv, (size_t)width * width * sizeof(float), false},
+                          {A, (size_t)vocab * sizeof(float), false},
+                          {damping, sizeof(float), false},
+                          {workspace, need, false}};
+  for (const Piece& a : pieces) {
+    KFAC_REQUIRE(a.p == workspace || aligned_to(a.p, sizeof(float)),
+                 "precondition_embedding: arrays not aligned to 4 bytes");
+    for (const Piece* b = &a + 1; b != pieces + 8; ++b)
+      KFAC_REQUIRE(!a.written || (a.p == kf && b->p == grad && kf == grad) ||
+                       !overlap(a.p, a.bytes, b->p, b->bytes),
+                   "precondition_embedding: what is written overlaps another array");
+  }
   char* ws = reinterpret_cast<char*>(
       (reinterpret_cast<uintptr_t>(workspace) + 255) & ~(uintptr_t)255);
   EmbedStep e = {};

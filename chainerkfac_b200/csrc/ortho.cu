@@ -21,6 +21,7 @@
 // Bound: the MMAs.  A step takes r^2 c + r^3 + 2 r^2 c flops, thrice with two terms.
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <exception>
 #include <vector>
 
@@ -550,6 +551,44 @@ static int check_shapes(int count, const int* rows, const int* cols) {
   return KFAC_OK;
 }
 
+// What a call writes may be what it reads of the same matrix, and nothing else: a
+// matrix may still be read, or be written by others, while one is written.
+static int check_apart(int count, const int* rows, const int* cols, size_t size,
+                       const Call& c) {
+  struct Piece {
+    uintptr_t begin, end;
+    int matrix;
+    bool written;
+  };
+  std::vector<Piece> all;
+  all.reserve(3 * (size_t)count);
+  auto add = [&](const void* p, int i, bool written) -> int {
+    if (p == nullptr) return KFAC_OK;
+    KFAC_REQUIRE(aligned_to(p, size), "orthogonalize: matrix %d is not aligned", i);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    all.push_back({at, at + (size_t)rows[i] * cols[i] * size, i, written});
+    return KFAC_OK;
+  };
+  for (int i = 0; i < count; ++i) {
+    int rc = add(c.x[i], i, false);
+    if (rc == KFAC_OK && c.out != nullptr) rc = add(c.out[i], i, true);
+    if (rc == KFAC_OK && c.param != nullptr) rc = add(c.param[i], i, true);
+    if (rc != KFAC_OK) return rc;
+  }
+  std::sort(all.begin(), all.end(),
+            [](const Piece& a, const Piece& b) { return a.begin < b.begin; });
+  for (size_t i = 0; i < all.size(); ++i)
+    for (size_t k = i + 1; k < all.size() && all[k].begin < all[i].end; ++k) {
+      const Piece &a = all[i], &b = all[k];
+      KFAC_REQUIRE((!a.written && !b.written) ||
+                       (a.written != b.written && a.matrix == b.matrix &&
+                        a.begin == b.begin),
+                   "orthogonalize: what is written of matrix %d overlaps matrix %d",
+                   a.written ? a.matrix : b.matrix, a.written ? b.matrix : a.matrix);
+    }
+  return KFAC_OK;
+}
+
 extern "C" size_t kfac_orthogonalize_workspace_bytes(int count, const int* rows,
                                                      const int* cols) {
   if (count <= 0 || check_shapes(count, rows, cols) != KFAC_OK) return 0;
@@ -581,12 +620,14 @@ extern "C" int kfac_orthogonalize(int dtype, int count, const int* rows,
                  "orthogonalize: matrix %d is null, or has nowhere to go", i);
   try {
     const Call c = {dtype, steps, coefficients, eps, lr, decay, x, out, param, scale};
-    if (all_small(count, rows, cols)) return run_small(count, rows, cols, c, stream);
     const size_t need = lay_out(count, rows, cols, nullptr, nullptr);
-    if (workspace == nullptr || workspace_bytes < need)
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
       return fail(KFAC_ERR_WORKSPACE,
                   "orthogonalize: %zu bytes of workspace, %zu needed",
                   workspace == nullptr ? (size_t)0 : workspace_bytes, need);
+    rc = check_apart(count, rows, cols, dtype == KFAC_WIRE_F32 ? 4 : 2, c);
+    if (rc != KFAC_OK) return rc;
+    if (need == 0) return run_small(count, rows, cols, c, stream);
     char* ws = reinterpret_cast<char*>(
         (reinterpret_cast<uintptr_t>(workspace) + 255) & ~(uintptr_t)255);
     std::vector<Shape> shapes;

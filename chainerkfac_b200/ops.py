@@ -830,6 +830,12 @@ def _chk_shape(t, shape, name):
             name, 'x'.join(str(v) for v in shape), tuple(t.shape)))
 
 
+def _c_int(n):
+    """A size as a C int: one that passes it as the largest there is, which the
+    library refuses (ctypes would cut it off)."""
+    return min(n, 0x7fffffff)
+
+
 def _scratch(nbytes, device):
     return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
 
@@ -862,7 +868,7 @@ def embedding(weight, ids, scale=1.0, ignore_label=None, out=None):
     _chk_place(index, ('ids', ids))
     has, label = _ignore(ignore_label)
     _lib.check(_lib.load().kfac_embedding(
-        WIRE_DTYPES[weight.dtype], weight.data_ptr(), vocab, width,
+        WIRE_DTYPES[weight.dtype], weight.data_ptr(), vocab, _c_int(width),
         ids.data_ptr(), ids.element_size(), ids.numel(), has, label, scale,
         out.data_ptr(), _raw_stream(index)), 'kfac_embedding')
     return out
@@ -943,13 +949,13 @@ def embedding_grad(gy, order, scale=1.0, out=None, accumulate=False):
     _chk_place(index, ('order', order), ('out', out))
     lib = _lib.load()
     n = order.count
-    nbytes = lib.kfac_embedding_grad_workspace_bytes(n, width)
+    nbytes = lib.kfac_embedding_grad_workspace_bytes(n, _c_int(width))
     ws = gy.new_empty(max(nbytes, 16), dtype=torch.uint8)
     stream = _raw_stream(index)
     order.used_on(stream)
     at = order.sorted.data_ptr()
     _lib.check(lib.kfac_embedding_grad(
-        WIRE_DTYPES[gy.dtype], gy.data_ptr(), width, at, at + 4 * n, n,
+        WIRE_DTYPES[gy.dtype], gy.data_ptr(), _c_int(width), at, at + 4 * n, n,
         order.vocab, scale, int(bool(accumulate)), out.data_ptr(),
         ws.data_ptr(), nbytes, stream), 'kfac_embedding_grad')
     return out
@@ -994,7 +1000,8 @@ def precondition_embedding(G_inv, A, damping, grad, kf=None, param=None,
     (vocab,), ``damping`` one element (a ``G_inv`` that lies column by column,
     as ``torch.linalg`` leaves it, is the same matrix).  With the weight ``param`` and its
     velocity ``mom``, mom = momentum * mom - lr * kf and param += mom as well.
-    Rows without a gradient get zeros in ``kf``, and cost no product."""
+    Rows without a gradient get zeros in ``kf`` (which may be ``grad`` itself), and
+    cost no product."""
     if G_inv.dim() == 2 and not G_inv.is_contiguous():
         G_inv = G_inv.t()
     for t, name in ((G_inv, 'G_inv'), (A, 'A'), (damping, 'damping'),
@@ -1024,9 +1031,9 @@ def precondition_embedding(G_inv, A, damping, grad, kf=None, param=None,
         kf = torch.empty_like(grad)
     lib = _lib.load()
     ws = _scratch(lib.kfac_precondition_embedding_workspace_bytes(
-        vocab, width), device)
+        vocab, _c_int(width)), device)
     _lib.check(lib.kfac_precondition_embedding(
-        vocab, width, G_inv.data_ptr(), A.data_ptr(), damping.data_ptr(),
+        vocab, _c_int(width), G_inv.data_ptr(), A.data_ptr(), damping.data_ptr(),
         grad.data_ptr(), kf.data_ptr(), _p(param), _p(mom), lr, momentum,
         ws.data_ptr(), ws.numel(), _stream()), 'kfac_precondition_embedding')
     return kf
@@ -1065,7 +1072,7 @@ def orthogonalize(xs, outs=None, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7,
     ``xs``: a tensor or a list (float32, float16 or bfloat16; the first
     dimension against all others: a convolution's weight is a matrix of
     filters); a list goes in one row of launches per type.  ``outs``: where to,
-    which may be ``xs``; ``scale``: a number, or one for each.  With weights
+    each of which may be its own x, and shares no memory with the others; ``scale``: a number, or one for each.  With weights
     ``params`` (of the same types)
     param = (1 - lr * decay) * param - lr * scale * X in the last product's
     epilogue; only ``outs`` that are given are then written."""
@@ -1112,8 +1119,9 @@ def orthogonalize(xs, outs=None, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7,
     for dtype, idx in groups.items():
         part = [xs[i] for i in idx]
         n = len(idx)
-        rows = (ctypes.c_int * n)(*[x.shape[0] for x in part])
-        cols = (ctypes.c_int * n)(*[x.numel() // x.shape[0] for x in part])
+        rows = (ctypes.c_int * n)(*[_c_int(x.shape[0]) for x in part])
+        cols = (ctypes.c_int * n)(*[_c_int(x.numel() // x.shape[0])
+                                    for x in part])
         for i in idx:
             if outs[i] is None and weights[i] is None:
                 outs[i] = torch.empty_like(xs[i])

@@ -504,7 +504,10 @@ int kfac_wire_unpack_sum_as(int wire_dtype, int n_arrays, float* const* arrays,
  * that weight.  Elements (weight, out, gy) are fp32, fp16 or bf16, `dtype`
  * numbered as the wire types above; sums are formed in fp32 and rounded once.
  * Matrices are row-major and dense, tokens 4- or 8-byte integers (`id_bytes`),
- * fewer than 2^31 - 4096 of them.  A token equal to `ignore` (has_ignore != 0)
+ * fewer than 2^31 - 4096 of them; rows have 1 .. 2^28 elements.  Arrays are
+ * aligned to their elements.  What a call writes shares no memory with its
+ * other arrays (refused), here and in the calls below, but where they say
+ * so.  A token equal to `ignore` (has_ignore != 0)
  * has no row: zeros in a lookup, nothing in a gradient or a count.  Neither
  * has one outside 0 .. vocab - 1: NaN in a lookup, nothing elsewhere.
  */
@@ -552,10 +555,11 @@ int kfac_token_counts(const void* ids, int id_bytes, int64_t n, int64_t vocab,
  * (X^T X and products from the right where rows exceed cols: the same values).
  * out[i] = scale[i] * X, and with a weight, param[i] of the same type,
  *     param = (1 - lr * decay) * param - lr * scale * X.
- * Either may be NULL, as arrays or element by element; out[i] may be x[i].
+ * Either may be NULL, as arrays or element by element; out[i] (or param[i])
+ * may be x[i].
  * fp32 products carry 22 bits of their operands; for 16-bit matrices whose
- * sides are both over 128, A and the polynomial carry 11.  An X with entries of 8 and more, or values that are
- * not finite, give NaN.  Pointer, size and coefficient arrays are host arrays
+ * sides are both over 128, A and the polynomial carry 11.  An X with entries
+ * of 8 and more, or values that are not finite, give NaN.  Pointer, size and coefficient arrays are host arrays
  * read during the call.  (Matrices with one side of up to 128 and the
  * other of up to 16 x 192 take one launch and no workspace, if all are.) */
 size_t kfac_orthogonalize_workspace_bytes(int count, const int* rows,
@@ -575,7 +579,7 @@ int kfac_orthogonalize(int dtype, int count, const int* rows, const int* cols,
  * symmetric matrix, and `damping` one device float (the value that the inverse
  * plan added to the diagonal of A's place).  With a weight and its velocity,
  *     mom = momentum * mom - lr * kf,   param = param + mom.
- * The pair may be NULL.  All fp32, dense, row-major.  Rows whose gradient
+ * The pair may be NULL; kf may be `grad`.  All fp32, dense, row-major.  Rows whose gradient
  * is zero have kf = 0 and cost no product; one with values that are not finite
  * gives NaN in its own row. */
 size_t kfac_precondition_embedding_workspace_bytes(int64_t vocab, int width);

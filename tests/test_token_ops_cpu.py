@@ -160,3 +160,74 @@ def test_precondition_embedding_calls_are_checked(lib):
     x = torch.zeros(3, 3)
     with pytest.raises(_lib.KfacLibraryError, match='CUDA tensor'):
         ops.precondition_embedding(x, x[0], x[0, :1], x)
+
+
+def test_results_do_not_overlap_what_is_read(lib):
+    at = ctypes.c_void_p
+    far = [at((k + 1) << 40) for k in range(9)]
+    look = lambda **k: lib.kfac_embedding(*({**dict(
+        dtype=0, weight=far[0], vocab=10, width=4, ids=far[1], id_bytes=8, n=5,
+        has=0, ignore=0, scale=1.0, out=far[2], stream=None), **k}).values())
+    for bad in (dict(out=far[0]), dict(out=at((1 << 40) + 156)),
+                dict(out=at((1 << 40) - 76)), dict(out=at((2 << 40) + 36))):
+        assert look(**bad) == 1, bad
+        assert 'overlaps' in message(lib)
+    order = lambda **k: lib.kfac_token_order(*({**dict(
+        ids=far[0], id_bytes=4, n=50, vocab=10, has=0, ignore=0, keys=far[1],
+        positions=far[2], ws=None, nbytes=0, stream=None), **k}).values())
+    for bad in (dict(keys=far[0]), dict(positions=far[0]),
+                dict(positions=at((2 << 40) + 196))):
+        assert order(**bad) == 1 and 'overlaps' in message(lib), bad
+    grad = lambda **k: lib.kfac_embedding_grad(*({**dict(
+        dtype=1, gy=far[0], width=8, keys=far[1], positions=far[2], n=100,
+        vocab=10, scale=1.0, accumulate=0, out=far[3], ws=far[4],
+        nbytes=1 << 30, stream=None), **k}).values())
+    for bad in (far[0], far[1], far[2], far[4], at((1 << 40) - 158)):
+        assert grad(out=bad) == 1 and 'overlaps' in message(lib), bad
+    counts = lambda **k: lib.kfac_token_counts(*({**dict(
+        ids=far[0], id_bytes=8, n=100, vocab=10, has=0, ignore=0, alpha=1.0,
+        beta=0.0, out=far[1], mean=far[2], ws=far[3], nbytes=40, stream=None),
+        **k}).values())
+    for bad in (dict(out=far[0]), dict(out=far[3]), dict(mean=far[1]),
+                dict(mean=far[0]), dict(mean=far[3])):
+        assert counts(**bad) == 1 and 'overlaps' in message(lib), bad
+    step = lambda **k: lib.kfac_precondition_embedding(*({**dict(
+        vocab=100, width=12, G=far[0], A=far[1], damping=far[2], grad=far[3],
+        kf=far[4], param=far[5], mom=far[6], lr=0.1, momentum=0.9, ws=far[7],
+        nbytes=1 << 30, stream=None), **k}).values())
+    for bad in (dict(kf=far[0]), dict(kf=far[1]), dict(kf=far[2]),
+                dict(kf=far[5]), dict(kf=at((4 << 40) + 4)), dict(mom=far[5]),
+                dict(mom=far[3]), dict(param=far[3]), dict(param=far[7])):
+        assert step(**bad) == 1 and 'overlaps' in message(lib), bad
+    big = 1 << 30
+    for bad in (dict(out=[8192, 8192]), dict(out=[8192, 4096]),
+                dict(out=[4100, big]), dict(out=None, param=[8192, 8192]),
+                dict(out=[8192, big], param=[8192, 2 * big]),
+                dict(out=[16384 + 4, big]), dict(out=[8192, 8192 + 92])):
+        got = ortho(lib, **{**dict(rows=[4, 4], cols=[6, 6], x=[4096, 16384],
+                                   scale=[1.0, 1.0]), **bad})
+        assert got == 1 and 'overlaps' in message(lib), bad
+
+
+def test_arrays_are_aligned_and_rows_have_a_size(lib):
+    at = ctypes.c_void_p
+    far = [at((k + 1) << 40) for k in range(9)]
+    odd = at((20 << 40) + 2)
+    for k in (dict(ids=at(4100)), dict(weight=odd), dict(out=odd),
+              dict(width=(1 << 28) + 1)):
+        assert lib.kfac_embedding(*({**dict(
+            dtype=0, weight=far[0], vocab=10, width=4, ids=far[1], id_bytes=8,
+            n=5, has=0, ignore=0, scale=1.0, out=far[2], stream=None),
+            **k}).values()) == 1, k
+        assert 'aligned' in message(lib) or '2^28' in message(lib)
+    assert ortho(lib, x=[4098]) == 1 and 'aligned' in message(lib)
+    assert ortho(lib, out=[4099], dtype=1) == 1 and 'aligned' in message(lib)
+    for name in ('G', 'A', 'damping', 'grad', 'kf'):
+        assert lib.kfac_precondition_embedding(*({**dict(
+            vocab=100, width=12, G=far[0], A=far[1], damping=far[2],
+            grad=far[3], kf=far[4], param=None, mom=None, lr=0.1, momentum=0.9,
+            ws=far[7], nbytes=1 << 30, stream=None), name: odd}).values()) == 1
+        assert 'aligned' in message(lib)
+    from chainerkfac_b200 import ops
+    assert ops._c_int(7) == 7
+    assert ctypes.c_int(ops._c_int(2 ** 32 + 5)).value == 2 ** 31 - 1

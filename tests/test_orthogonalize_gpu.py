@@ -290,3 +290,55 @@ def test_replayed_and_on_two_streams():
     status = _lib.ctypes.c_int(7)
     _lib.check(_lib.load().kfac_tc_status(_lib.ctypes.byref(status)), 'status')
     assert status.value == 0
+
+
+def test_the_same_matrix_twice_and_a_weight_twice():
+    from chainerkfac_b200 import _lib, ops
+    x = torch.randn((300, 140), device='cuda', generator=gen(1))
+    a, b = ops.orthogonalize([x, x], scale=[1.0, 2.0])
+    check(a, x)
+    assert torch.equal(2 * a, b)
+    w = torch.zeros_like(x)
+    for call in (lambda: ops.orthogonalize([x, x], params=[w, w], lr=0.1),
+                 lambda: ops.orthogonalize([x, a], outs=[a, b]),
+                 lambda: ops.orthogonalize([x, x[:64]], outs=[x, b[:64]])):
+        with pytest.raises(_lib.KfacLibraryError, match='overlaps'):
+            call()
+    assert not w.any()
+
+
+def test_calls_from_threads():
+    """Several threads at once, a stream each, small and large matrices and an
+    embedding's step in between."""
+    import threading
+    from chainerkfac_b200 import ops
+    xs = [torch.randn(s, device='cuda', generator=gen(k)) for k, s in
+          enumerate([(64, 147), (100, 900), (300, 260), (520, 390)])]
+    G_inv = torch.eye(130, device='cuda')
+    A, damping = torch.ones(700, device='cuda'), torch.ones(1, device='cuda')
+    grad = torch.randn((700, 130), device='cuda', generator=gen(9))
+
+    def work(x):
+        return (ops.orthogonalize(x),
+                ops.precondition_embedding(G_inv, A, damping, grad))
+    want = [work(x) for x in xs]
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def run(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                got[k] = [work(xs[k]) for _ in range(10)]
+            stream.synchronize()
+        except Exception as e:                     # shown below
+            errors.append(e)
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for k, w in enumerate(want):
+        for g in got[k]:
+            assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])

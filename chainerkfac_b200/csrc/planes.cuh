@@ -190,18 +190,17 @@ __device__ __forceinline__ void pl_load(unsigned dst, const CUtensorMap* map, in
       : "memory");
 }
 
-// One term of an operand tile: rows r0.. of it, k-block kb.  Rows down the planes: a
-// box of 128 rows x 64 k; rows along the planes: two boxes of 64 k x 64 rows.
+// The terms of an operand tile, from (x, y) of its planes.  Rows down the planes: a box
+// of 128 rows x 64 k; rows along them (`mn`): two boxes of 64 k x 64 rows.
 template <int G>
-__device__ __forceinline__ void pl_load_term(unsigned dst, const CUtensorMap* map,
-                                             int mn, int r0, int kb, int term,
-                                             unsigned bar) {
-  if (!mn) {
-    pl_load<G>(dst, map, kb * PL_BK, r0, term, bar);
-  } else {
-    pl_load<G>(dst, map, r0, kb * PL_BK, term, bar);
-    pl_load<G>(dst + PL_TERM / 2, map, r0 + 64, kb * PL_BK, term, bar);
-  }
+__device__ __forceinline__ void pl_load_terms(unsigned dst, const CUtensorMap* map,
+                                              bool mn, int x, int y, int terms,
+                                              unsigned bar) {
+  pl_load<G>(dst, map, x, y, 0, bar);
+  if (mn) pl_load<G>(dst + PL_TERM / 2, map, x + 64, y, 0, bar);
+  if (terms < 2) return;
+  pl_load<G>(dst + PL_TERM, map, x, y, 1, bar);
+  if (mn) pl_load<G>(dst + PL_TERM + PL_TERM / 2, map, x + 64, y, 1, bar);
 }
 
 // Two values as fp16 terms, rounded to nearest.  Beyond the range hi is infinite and
@@ -444,47 +443,55 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
     counted = *reinterpret_cast<const volatile int*>(l.rows);
     tiles = (counted + TILE - 1) / TILE * l.p[0].f.tiles_n;
   }
+  // (The loops over k-blocks carry stages, phases, coordinates and descriptors along:
+  // a k-block of one product is in the tensor cores for 512 cycles, and with divisions
+  // and addresses made anew each of the two threads took 500 and more for one, waits
+  // aside.)
   if (warp == 0) {
     if (elect_one()) {
-      int it = 0;
-      bool ok = true;
+      int s = 0;
+      unsigned turn = 1;                     // (the first round finds all stages empty)
+      bool ok = true, begun = false;
+      // both CTAs' loads count at the first one's barrier
+      const unsigned own = smem_u32(ctl->full), bars = cluster_addr(own, first);
+      const unsigned stage0 = smem_u32(smem);
       for (int tile = tile0; ok && tile < tiles; tile += step) {
         const PlaneProblem& p = pl_problem(l, tile);
         const PlaneFields g = p.f;
         int m0, n0, kb0, nkb;
         pl_tile_at<G>(g, tile, m0, n0);
         range(g, kb0, nkb);
-        const bool share = g.same && m0 == n0;
+        const bool share = g.same && m0 == n0, amn = g.a_mn, bmn = g.b_mn;
         const int ta = g.ta, tb = g.tb;
-        const unsigned bytes = (share ? ta : ta + tb) * PL_TERM;
+        const unsigned bytes = G * (share ? ta : ta + tb) * PL_TERM;
         const int ra = m0 + PL_ROWS * side, rb = n0 + PL_ROWS * side;
-        if (it == 0) {
+        int k = kb0 * PL_BK;
+        if (!begun) {
+          begun = true;
           asm volatile("prefetch.tensormap [%0];" ::"l"(&p.ma) : "memory");
           asm volatile("prefetch.tensormap [%0];" ::"l"(&p.mb) : "memory");
           wait_for_launch_before();
           // what it wrote is read by the copy engine
           asm volatile("fence.proxy.async;" ::: "memory");
         }
-        for (int kb = kb0; kb < kb0 + nkb; ++kb, ++it) {
-          const int s = it % stages;
-          if (it >= stages &&
-              !mbar_wait_status(&ctl->empty[s], ((it / stages) - 1) & 1,
-                                &ctl->abort_flag, status)) {
+        for (int kb = 0; kb < nkb; ++kb, k += PL_BK) {
+          if (!mbar_wait_status(&ctl->empty[s], turn, &ctl->abort_flag, status)) {
             ok = false;
             break;
           }
-          // both CTAs' loads count at the first one's barrier
-          const unsigned bar = cluster_addr(smem_u32(&ctl->full[s]), first);
+          const unsigned bar = bars + 8 * s, st = stage0 + s * stage_bytes;
           if (side == 0)
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-                         ::"r"(smem_u32(&ctl->full[s])), "r"(G * bytes)
+                         ::"r"(own + 8 * s), "r"(bytes)
                          : "memory");
-          const unsigned st = smem_u32(smem + s * stage_bytes);
-          for (int t = 0; t < ta; ++t)
-            pl_load_term<G>(st + t * PL_TERM, &p.ma, g.a_mn, ra, kb, t, bar);
-          if (share) continue;
-          for (int t = 0; t < tb; ++t)
-            pl_load_term<G>(st + (ta + t) * PL_TERM, &p.mb, g.b_mn, rb, kb, t, bar);
+          pl_load_terms<G>(st, &p.ma, amn, amn ? ra : k, amn ? k : ra, ta, bar);
+          if (!share)
+            pl_load_terms<G>(st + ta * PL_TERM, &p.mb, bmn, bmn ? rb : k,
+                             bmn ? k : rb, tb, bar);
+          if (++s == stages) {
+            s = 0;
+            turn ^= 1;
+          }
         }
       }
     }
@@ -494,8 +501,10 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
     wait_for_launch_before();
     if (side == 0 && elect_one()) {
       const unsigned short both = (unsigned short)(3u << first);
-      int it = 0, seg = 0;
+      int s = 0, seg = 0;
+      unsigned turn = 0;
       bool ok = true;
+      const unsigned stage0 = smem_u32(smem);
       for (int tile = tile0; ok && tile < tiles; tile += step) {
         const PlaneFields g = pl_problem(l, tile).f;
         int m0, n0, kb0, nkb;
@@ -509,9 +518,13 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
         const unsigned long long adv_a = (amn ? 2048 : 32) >> 4;
         const unsigned long long adv_b = (bmn ? 2048 : 32) >> 4;
         const unsigned long long lo = PL_TERM >> 4;
+        const unsigned stage_b = share ? stage0 : stage0 + ta * PL_TERM;
+        const unsigned long long a0 =
+            amn ? tc_smem_desc_mn(stage0, PL_TERM / 2) : tc_smem_desc(stage0);
+        const unsigned long long b0 =
+            bmn ? tc_smem_desc_mn(stage_b, PL_TERM / 2) : tc_smem_desc(stage_b);
         unsigned d = 0;
-        for (int kb = 0; kb < nkb; ++kb, ++it) {
-          const int s = it % stages;
+        for (int kb = 0; kb < nkb; ++kb) {
           const bool fresh = kb == 0 || (cut && kb % PL_SEGMENT == 0);
           if (fresh) {
             const int b = seg & 1;
@@ -523,18 +536,13 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
               break;
             }
           }
-          if (!mbar_wait_status(&ctl->full[s], (it / stages) & 1, &ctl->abort_flag,
-                                status)) {
+          if (!mbar_wait_status(&ctl->full[s], turn, &ctl->abort_flag, status)) {
             ok = false;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const unsigned sa = smem_u32(smem + s * stage_bytes);
-          const unsigned sb = share ? sa : sa + ta * PL_TERM;
-          const unsigned long long a =
-              amn ? tc_smem_desc_mn(sa, PL_TERM / 2) : tc_smem_desc(sa);
-          const unsigned long long b =
-              bmn ? tc_smem_desc_mn(sb, PL_TERM / 2) : tc_smem_desc(sb);
+          const unsigned long long at = (unsigned)(s * stage_bytes) >> 4;
+          const unsigned long long a = a0 + at, b = b0 + at;
           unsigned acc = !fresh;
           if (G == 1) {
 #pragma unroll
@@ -570,6 +578,10 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
           if (kb + 1 == nkb || (cut && (kb + 1) % PL_SEGMENT == 0)) {
             pl_commit<G>(&ctl->accum[seg & 1], both);
             ++seg;
+          }
+          if (++s == stages) {
+            s = 0;
+            turn ^= 1;
           }
         }
       }

@@ -10,9 +10,7 @@
 // along the rows or down the columns of the planes, and fills zeros past the edges, so
 // any size goes without a copy.  In each CTA warp 0 issues the loads and, in the first
 // of a pair, warp 1 the MMAs; eight warps take the accumulators, which are there twice,
-// out of tensor memory while the MMAs go on in the other one.  An MMA of 128 columns
-// takes 150 cycles behind one on the same accumulator instead of 64, one of 256 its
-// 128: the small tiles have cross terms in an accumulator of their own.
+// out of tensor memory while the MMAs go on in the other one.
 //
 // The tensor core adds with truncation, so a long sum comes out too small by what
 // its number of additions makes: a sum of two-term products is cut every PL_SEGMENT
@@ -58,6 +56,7 @@ constexpr int PL_SMEM =
 constexpr int PL_COLS = 512;                 // tensor memory: two accumulators
 // Cycles of an MMA of 128 columns, and what a small tile takes beside its MMAs with a
 // shared sum and without (plane_split).
+constexpr double PL_FEED = 6600;             // bytes a cycle that all SMs get from L2
 constexpr double PL_SMALL_MMA = 85, PL_SMALL_SHARE = 5000, PL_SMALL_END = 5000;
 static_assert(PL_ROWS * 256 * 4 <= PL_STAGE_BYTES, "parts of a shared sum");
 
@@ -394,7 +393,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int stage_bytes = l.terms * PL_TERM;
   const int stages = PL_STAGE_BYTES / stage_bytes;
-  const bool cut = l.terms == 4, cross = G == 1 && l.terms > 2;
+  const bool cut = l.terms == 4;
   const int S = l.split;
   const unsigned rank = cluster_rank(), side = rank % G, first = rank - side;
   const int part = (int)(rank / G);                // of a shared sum
@@ -544,35 +543,24 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
           const unsigned long long at = (unsigned)(s * stage_bytes) >> 4;
           const unsigned long long a = a0 + at, b = b0 + at;
           unsigned acc = !fresh;
-          if (G == 1) {
+          if (tb == 2) {
 #pragma unroll
             for (int kk = 0; kk < PL_BK / 16; ++kk) {
-              const unsigned long long ak = a + kk * adv_a, bk = b + kk * adv_b;
-              if (tb == 2) pl_mma<G>(d + TILE, ak, bk + lo, idesc, acc);
-              pl_mma<G>(d, ak, bk, idesc, acc);
-              if (ta == 2) pl_mma<G>(d + TILE, ak + lo, bk, idesc, acc | (tb == 2));
+              pl_mma<G>(d, a + kk * adv_a, b + lo + kk * adv_b, idesc, acc);
               acc = 1;
             }
-          } else {
-            if (tb == 2) {
-#pragma unroll
-              for (int kk = 0; kk < PL_BK / 16; ++kk) {
-                pl_mma<G>(d, a + kk * adv_a, b + lo + kk * adv_b, idesc, acc);
-                acc = 1;
-              }
-            }
-            if (ta == 2) {
-#pragma unroll
-              for (int kk = 0; kk < PL_BK / 16; ++kk) {
-                pl_mma<G>(d, a + lo + kk * adv_a, b + kk * adv_b, idesc, acc);
-                acc = 1;
-              }
-            }
+          }
+          if (ta == 2) {
 #pragma unroll
             for (int kk = 0; kk < PL_BK / 16; ++kk) {
-              pl_mma<G>(d, a + kk * adv_a, b + kk * adv_b, idesc, acc);
+              pl_mma<G>(d, a + lo + kk * adv_a, b + kk * adv_b, idesc, acc);
               acc = 1;
             }
+          }
+#pragma unroll
+          for (int kk = 0; kk < PL_BK / 16; ++kk) {
+            pl_mma<G>(d, a + kk * adv_a, b + kk * adv_b, idesc, acc);
+            acc = 1;
           }
           pl_commit<G>(&ctl->empty[s], both);
           if (kb + 1 == nkb || (cut && (kb + 1) % PL_SEGMENT == 0)) {
@@ -623,15 +611,6 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
           float x[16], y[16];
           tc_ld_16x32(at + 32 * u, x);
           tc_ld_16x32(at + (16u << 16) + 32 * u, y);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            v[32 * u + i] += x[i];
-            v[32 * u + 16 + i] += y[i];
-          }
-          if (!cross) continue;
-          tc_ld_16x32(at + TILE + 32 * u, x);
-          tc_ld_16x32(at + (16u << 16) + TILE + 32 * u, y);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -768,11 +747,10 @@ inline int plane_map(CUtensorMap* map, const Planes& o, int rows, int cols, bool
 // the 4 n others 1 / 4n, 2 / 4n .. 1: 6 n - 3.5 whole ones.  Errors of orthogonalised
 // 4096 x 4096 and 1024 x 4096 against fp64, with and without:
 // 1.9e-6 and 3.0e-6, 2.3e-6 and 4.0e-6 (fp32 products: 4.3e-6, 3.7e-6).
-// (Small tiles have the cross terms elsewhere: 2 n + 0.5.)
-inline float plane_gain(int terms, int K, int G) {
+inline float plane_gain(int terms, int K) {
   if (terms < 4) return 1.f;
   const int n = std::min((K + PL_BK - 1) / PL_BK, PL_SEGMENT);
-  return 1.f + (G == 2 ? 6 * n - 3.5f : 2 * n + 0.5f) * 0.72f * exp2f(-24);
+  return 1.f + (6 * n - 3.5f) * 0.72f * exp2f(-24);
 }
 
 // Numbers the tiles of l.p[0 .. l.n), of G blocks each.
@@ -786,7 +764,7 @@ void plane_number_tiles(PlaneLaunch<N>& l, int G) {
     g.tiles_n = tn;
     g.tile_begin = total;
     total += g.lower ? tm * (tm + 1) / 2 : tm * tn;
-    g.gain = plane_gain(g.ta + g.tb, g.K, G);
+    g.gain = plane_gain(g.ta + g.tb, g.K);
   }
   l.tiles = total;
   l.terms = l.n > 0 ? l.p[0].f.ta + l.p[0].f.tb : 0;
@@ -794,41 +772,49 @@ void plane_number_tiles(PlaneLaunch<N>& l, int G) {
 
 // Small tiles or large ones, and how many blocks or pairs share one: what a count of
 // cycles comes out least for, with `room[i]` clusters of 2^i of them on the GPU at a
-// time.  A k-block takes an MMA of 128 cycles (small tiles 85, or 150 behind each other)
-// for each 16 k and product of terms; a tile's start and end 11000 (small 7000; beside
-// the next one's MMAs 2000), with a shared sum 8000 (5000) and 500 for each that shares:
-// the parts go through distributed shared memory at 20 bytes a cycle and SM, but each
-// has a part of the epilogue only.  Five steps, us so, and with large tiles only: 256 x
-// 512 139 and 194, 512 x 512 155 and 215, 1000 x 1000 242 and 279, 512 x 4608 232 and
-// 293, one matrix of each kind of ResNet-50 464 and 520; with small tiles only 1024 x
-// 4096 412 (378 so), 2048 x 2048 625 (578).
+// time.  A k-block takes an MMA of 128 cycles (small tiles 85 for 64: their operands and
+// the copies into their place want more of the shared memory than its 128 bytes a cycle;
+// 110 of one product) for each 16 k and product of terms; all SMs together get no more
+// than PL_FEED bytes a cycle from L2, and small tiles want twice as many; a tile's start
+// and end 11000 (small 7000; beside the next one's MMAs 2000), with a shared sum 8000
+// (5000) and 500 for each that shares: the parts go through distributed shared memory at
+// 20 bytes a cycle and SM, but each has a part of the epilogue only.  Five steps, us so,
+// with large tiles only, with small ones only: 256 x 512 137, 189, 136; 1000 x 1000
+// 238, 273, 239; 512 x 4608 220, 282, 220; 1024 x 4096 364, 367, 390; 2048 x 2048 556,
+// 679, 590; one matrix of each kind of ResNet-50 450, 509, 458; all 54 of it 1234,
+// 1292, 1273; 8191 x 2047 bf16 856, 856, 1062 (and without PL_FEED 902).
 struct PlaneShape {
   int G, split;
   double cycles;
 };
 template <int N>
 void plane_split(const PlaneLaunch<N>& l, int G, const int* room, PlaneShape& best) {
-  // of a k-block: MMAs of 256 columns, or of 128 in one or two accumulators
+  // of a k-block
   const double cycles = G == 2           ? (l.terms - 1) * 4 * 132.0
-                        : l.terms == 2 ? 4 * 150.0
+                        : l.terms == 2 ? 4 * 110.0
                                        : (l.terms - 1) * 4 * PL_SMALL_MMA;
   for (int i = 0, s = 1; i < 4 && s <= (G == 2 ? 8 : 4); ++i, s *= 2) {
     if (room[i] <= 0) break;
     const double more = s > 1 ? (G == 2 ? 8000 : PL_SMALL_SHARE) + 500 * s : 2000;
-    double longest = 0, sum = 0;
+    double longest = 0, sum = 0, bytes = 0;
     for (int k = 0; k < l.n; ++k) {
       const int end = k + 1 < l.n ? l.p[k + 1].f.tile_begin : l.tiles;
       const int kb = (l.p[k].f.K + PL_BK - 1) / PL_BK;
+      bytes += (double)kb * (end - l.p[k].f.tile_begin) * l.terms * PL_TERM * G;
       const double one = (kb + s - 1) / s * cycles + more;
       longest = std::max(longest, one);
       sum += one * (end - l.p[k].f.tile_begin);
     }
-    // (tiles of one size run in whole waves, of different sizes closer together)
+    // (tiles of one size run in whole waves, of different sizes closer together, with
+    // one's start and end beside the other's k-blocks)
     const double waves = (double)l.tiles / room[i];
-    const double time =
-        std::max(longest, l.n == 1 ? sum / l.tiles * std::ceil(waves)
-                                   : sum / l.tiles * waves + longest / 2) +
-        (s > 1 ? 0 : G == 2 ? 9000 : PL_SMALL_END);
+    double busy = sum / l.tiles * waves + longest / 2, feed = bytes / PL_FEED;
+    if (l.n == 1) {
+      busy = sum / l.tiles * std::ceil(waves);
+      feed += more * std::ceil(waves);
+    }
+    const double time = std::max(std::max(longest, busy), feed) +
+                        (s > 1 ? 0 : G == 2 ? 9000 : PL_SMALL_END);
     if (best.G == 0 || time < best.cycles) best = {G, s, time};
   }
 }

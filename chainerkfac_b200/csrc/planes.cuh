@@ -58,7 +58,7 @@ constexpr int PL_COLS = 512;                 // tensor memory: two accumulators
 // shared sum and without (plane_split).
 constexpr double PL_FEED = 6600;             // bytes a cycle that all SMs get from L2
 constexpr double PL_SMALL_MMA = 85, PL_SMALL_SHARE = 5000, PL_SMALL_END = 5000;
-static_assert(PL_ROWS * 256 * 4 <= PL_STAGE_BYTES, "parts of a shared sum");
+static_assert(256 * 512 <= PL_STAGE_BYTES, "parts of a shared sum");
 
 // A pair of planes.
 struct Planes {
@@ -430,6 +430,14 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
   // (each role waits for the launch before where it first reads or writes memory)
 
   const unsigned tmem = ctl->tmem_base;
+  // Parts of a shared sum go to the end of the stages; where no k-block of the tile lies
+  // there, nobody has to wait for the others' MMAs before writing them.
+  constexpr int PARTS = TILE * 512;
+  bool apart = true;
+  if (S > 1) {
+    const int all = (pl_problem(l, tile0).f.K + PL_BK - 1) / PL_BK;
+    apart = (all + S - 1) / S * stage_bytes <= PL_STAGE_BYTES - PARTS;
+  }
   // k-blocks of a tile that this pair adds up
   auto range = [&](const PlaneFields& g, int& kb0, int& nkb) {
     const int all = (g.K + PL_BK - 1) / PL_BK, each = (all + S - 1) / S;
@@ -471,7 +479,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
           asm volatile("prefetch.tensormap [%0];" ::"l"(&p.mb) : "memory");
           wait_for_launch_before();
           // what it wrote is read by the copy engine
-          asm volatile("fence.proxy.async;" ::: "memory");
+          asm volatile("fence.proxy.async.global;" ::: "memory");
         }
         for (int kb = 0; kb < nkb; ++kb, k += PL_BK) {
           if (!mbar_wait_status(&ctl->empty[s], turn, &ctl->abort_flag, status)) {
@@ -628,8 +636,9 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
         // each, a multiple of the 32 that 32 registers hold.  Parts lie by pair, rows'
         // quarter, four registers, lane.
         const int width = TILE / S, groups = width / 4;
-        const unsigned base = smem_u32(smem);
-        cluster_sync();                      // the MMAs have read all stages
+        unsigned char* const parts = smem + PL_STAGE_BYTES - PARTS;
+        const unsigned base = smem_u32(parts);
+        if (!apart) cluster_sync();          // the MMAs have read all stages
         if (ok) {
 #pragma unroll
           for (int i = 0; i < COLS / 4; ++i) {
@@ -657,7 +666,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
 #pragma unroll 1
           for (int p = 0; p < S; ++p) {
             const unsigned char* from =
-                smem + ((p * 4 + q) * groups + c0 / 4) * 512 + lane * 16;
+                parts + ((p * 4 + q) * groups + c0 / 4) * 512 + lane * 16;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float4 w = *reinterpret_cast<const float4*>(from + 512 * i);
@@ -684,13 +693,13 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
     }
   }
   if (S > 1 && warp < 4) {
-    cluster_sync();
+    if (!apart) cluster_sync();
     cluster_sync();
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   // (nobody leaves while the other may still arrive at its barriers)
-  cluster_sync();
+  if (G == 2) cluster_sync();
   using Columns = typename std::conditional<G == 2, PairColumns, unsigned>::type;
   if (warp == 1) tc_release(tmem, Columns{PL_COLS}, ctl->abort_flag != 0);
 }

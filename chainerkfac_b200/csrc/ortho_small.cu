@@ -10,12 +10,12 @@
 //
 // X lies in tiles of 128 rows x 64 columns, 128 bytes a row: the layout that the MMAs
 // read as rows of k (A = X X^T) and as columns of k (B X) alike, so a step never moves
-// X.  A matrix that is taller than wide is turned when it is read.  Every product of
-// terms has an accumulator of its own (A's lo * hi and hi * lo as well), so that the MMAs
-// do not wait for each other; a sum is at most 256 k long.
+// X.  A matrix that is taller than wide is turned when it is read.  A sum is at most 256
+// k long, with the cross terms of all of them first.
 //
-// Bound: latency.  Five steps: 64 x 147 39 us (15 launches 150), 128 x 256 65, 64 x 576
-// 51, 128 x 1152 88 us.
+// Bound: latency.  Five steps: 64 x 147 32 us (15 launches 150), 128 x 256 57, 64 x 576
+// 48, 128 x 1152 81 us.  (With an accumulator for every product of terms, which the MMAs
+// do not need to stay apart, 36, 62, 50 and 86.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -99,8 +99,8 @@ __device__ __forceinline__ void os_add(unsigned planes, int r0, int c0, int lane
   }
 }
 
-// v = the sum of `n` accumulators 32 x 32, `apart` columns from each other.
-__device__ __forceinline__ void os_sums(unsigned at, int n, int apart, float (&v)[32]) {
+// v = 32 x 32 of an accumulator.
+__device__ __forceinline__ void os_sums(unsigned at, float (&v)[32]) {
   float x[16], y[16];
   tc_ld_16x32(at, x);
   tc_ld_16x32(at + (16u << 16), y);
@@ -109,17 +109,6 @@ __device__ __forceinline__ void os_sums(unsigned at, int n, int apart, float (&v
   for (int i = 0; i < 16; ++i) {
     v[i] = x[i];
     v[16 + i] = y[i];
-  }
-#pragma unroll 1
-  for (int k = 1; k < n; ++k) {
-    tc_ld_16x32(at + k * apart, x);
-    tc_ld_16x32(at + k * apart + (16u << 16), y);
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      v[i] += x[i];
-      v[16 + i] += y[i];
-    }
   }
 }
 
@@ -170,7 +159,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
   if (warp == 0) {
     asm volatile(
         "tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-        ::"r"(smem_u32(&ctl->tmem_base)), "r"(512)
+        ::"r"(smem_u32(&ctl->tmem_base)), "r"(256)
         : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;"
                  ::: "memory");
@@ -236,9 +225,10 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
     os_store16(to + OS_PLANE, lo);
   }
 
-  // Two terms of everything, for 16-bit matrices too: the launch takes little longer
-  // (64 x 147 bf16 39 us, with one 30), and of a matrix with few rows the rounding of A and B to one
-  // would be more than the result's own (385 x 33 fp16: 3.1e-3 of it).
+  // Two terms of everything, for 16-bit matrices too: of a matrix with few rows the
+  // rounding of A and B to one would be more than the result's own (385 x 33 fp16:
+  // 3.1e-3 of it); 64 x 147 bf16 took 39 us with two and 30 with one, before the sums
+  // of all products of terms shared an accumulator.
   constexpr int terms = 2;
   const int nk = (r + 15) >> 4, ck = (c + 15) >> 4;
   const int q = warp & 3, h = warp >> 2, r0 = 32 * q;
@@ -263,6 +253,21 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
     phase ^= 1;
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   };
+  // planes times themselves over n times 16 k, cross terms first, while the sum is small
+  auto square = [](unsigned tmem, unsigned planes, int n, unsigned idesc) {
+    const unsigned long long lo = OS_PLANE >> 4;
+    for (int k = 0; k < n; ++k) {
+      const unsigned long long a =
+          tc_smem_desc(planes + (k >> 2) * OS_TILE) + (k & 3) * 2;
+      tc_mma_half(tmem, a, a + lo, idesc, k != 0);
+      tc_mma_half(tmem, a + lo, a, idesc, 1);
+    }
+    for (int k = 0; k < n; ++k) {
+      const unsigned long long a =
+          tc_smem_desc(planes + (k >> 2) * OS_TILE) + (k & 3) * 2;
+      tc_mma_half(tmem, a, a, idesc, 1);
+    }
+  };
   // of a sum of n additions that truncate, on average (see plane_gain)
   auto gain = [](int n) { return 1.f + 0.36f * (n + 1) * exp2f(-24); };
 
@@ -272,16 +277,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
     // A = X X^T
     product([&]() {
       const unsigned idesc = tc_half_desc(16 * nk, false, false);
-      for (int k = 0; k < ck; ++k) {
-        const unsigned long long a =
-            tc_smem_desc(X + (k >> 2) * OS_TILE) + (k & 3) * 2;
-        const unsigned long long lo = OS_PLANE >> 4;
-        tc_mma_half(tmem, a, a, idesc, k != 0);
-        if (terms == 2) {
-          tc_mma_half(tmem + 128, a, a + lo, idesc, k != 0);
-          tc_mma_half(tmem + 256, a + lo, a, idesc, k != 0);
-        }
-      }
+      square(tmem, X, ck, idesc);
     });
     const float make_a = exp2f(kAExp - 2 * kXExp) * gain(ck);
     const int squares = (r + 31) >> 5;       // a side of A, in units
@@ -289,7 +285,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
 #pragma unroll 1
       for (int c0 = 32 * h; c0 < r; c0 += 32 * OS_WARPS / 4) {
         float v[32];
-        os_sums(quarter + c0, 2 * terms - 1, 128, v);
+        os_sums(quarter + c0, v);
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = ck > 0 ? v[i] * make_a : 0.f;
         if constexpr (!SPLIT) {
@@ -354,25 +350,16 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
     // B = a I + b A + c A A, in A's place
     product([&]() {
       const unsigned idesc = tc_half_desc(16 * nk, false, false);
-      for (int k = 0; k < nk; ++k) {
-        const unsigned long long a =
-            tc_smem_desc(A + (k >> 2) * OS_TILE) + (k & 3) * 2;
-        const unsigned long long lo = OS_PLANE >> 4;
-        tc_mma_half(tmem, a, a, idesc, k != 0);
-        if (terms == 2) {
-          tc_mma_half(tmem + 128, a, a + lo, idesc, k != 0);
-          tc_mma_half(tmem + 256, a + lo, a, idesc, k != 0);
-        }
-      }
+      square(tmem, A, nk, idesc);
     });
-    const float square = k3[2] * exp2f(-kAExp) * gain(nk), diag = k3[0] * exp2f(kAExp);
+    const float cube = k3[2] * exp2f(-kAExp) * gain(nk), diag = k3[0] * exp2f(kAExp);
     if (r0 < r) {
 #pragma unroll 1
       for (int c0 = 32 * h; c0 < r; c0 += 32 * OS_WARPS / 4) {
         float v[32];
-        os_sums(quarter + c0, 2 * terms - 1, 128, v);
+        os_sums(quarter + c0, v);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] *= square;
+        for (int i = 0; i < 32; ++i) v[i] *= cube;
         os_add(A, r0, c0, lane, k3[1], v, terms);
         if (c0 == r0) {
           const int d = 2 * (lane & 3) - (lane >> 2);
@@ -396,10 +383,12 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
             tc_smem_desc(A + (k >> 2) * OS_TILE) + (k & 3) * 2;
         const unsigned long long b = tc_smem_desc_mn(X + k * 2048, OS_TILE);
         const unsigned long long lo = OS_PLANE >> 4;
-        tc_mma_half(tmem, a, b, idesc, k != 0);
-        tc_mma_half(tmem + 256, a, b + lo, idesc, k != 0);
-        if (terms == 2) tc_mma_half(tmem + 256, a + lo, b, idesc, 1);
+        tc_mma_half(tmem, a, b + lo, idesc, k != 0);
+        tc_mma_half(tmem, a + lo, b, idesc, 1);
       }
+      for (int k = 0; k < nk; ++k)
+        tc_mma_half(tmem, tc_smem_desc(A + (k >> 2) * OS_TILE) + (k & 3) * 2,
+                    tc_smem_desc_mn(X + k * 2048, OS_TILE), idesc, 1);
     });
     const bool last = step + 1 == l.steps;
     const float make_x =
@@ -408,7 +397,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
 #pragma unroll 1
     for (int c0 = 32 * h; c0 < c; c0 += 32 * OS_WARPS / 4) {
       float v[32];
-      os_sums(quarter + c0, 2, 256, v);
+      os_sums(quarter + c0, v);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] *= make_x;
       if (!last) {
@@ -441,7 +430,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (warp == 0) tc_release(ctl->tmem_base, 512u, ctl->abort_flag != 0);
+  if (warp == 0) tc_release(ctl->tmem_base, 256u, ctl->abort_flag != 0);
 }
 
 template <typename T, bool SPLIT>

@@ -13,7 +13,10 @@
 // the result, while an error of X is relative to its largest singular value and grows
 // with the smallest ones (485 times in five steps of the usual coefficients): X keeps
 // two.  Simulated at 512 x 2048 (Gaussian with a part of low rank), error before the
-// last rounding: 1e-3 so, 4e-3 and more with one term of X, 1e-2 with bf16 ones.
+// last rounding: 1e-3 so, 4e-3 and more with one term of X, 1e-2 with bf16 ones.  Near
+// its diagonal, where its errors are those of whole rows of X, B has two as well.
+// Simulated at 512 x 4608 (Gaussian): 1.6e-3 without, 8e-4 so, and no less with two
+// everywhere.
 //
 // Entries of 8 and more in X (16 in A and B) are out of range and give NaN; the
 // usual coefficients keep X below 1.3.
@@ -175,6 +178,7 @@ struct EpiPlanes {
   float alpha, beta, diag;
   int terms;
   bool poly;
+  bool near;             // two terms near the diagonal (in blocks of 256)
   __device__ __forceinline__ NothingAhead begin(const PlaneFields&,
                                                 const PlaneTile&) const {
     return NothingAhead();
@@ -234,7 +238,8 @@ struct EpiPlanes {
             v[i] += diag;
       }
     }
-    pl_store_planes(t, g.out, v, g.M, g.N, terms, mirror);
+    const bool both = near && (t.r0 >> 8) == (t.c0 >> 8);
+    pl_store_planes(t, g.out, v, g.M, g.N, both ? 2 : terms, mirror);
   }
 };
 
@@ -484,6 +489,7 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
       q.b_mn = !tall;
       q.ta = tall ? 2 : terms;
       q.tb = tall ? terms : 2;
+      q.near = terms == 2 ? 0 : tall ? 2 : 1;
       q.out = m.x[k ^ 1];
     }
     poly.p[i].ma = poly.p[i].mb = a;
@@ -504,15 +510,15 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
   for (int step = 0; step < c.steps; ++step) {
     const float* k = c.coefficients + 3 * step;
     const int from = step & 1;
-    const EpiPlanes make_a = {exp2f(kAExp - 2 * kXExp), 0.f, 0.f, terms, false};
+    const EpiPlanes make_a = {exp2f(kAExp - 2 * kXExp), 0.f, 0.f, terms, false, false};
     rc = plane_launch("ortho X X^T", gram[from], make_a, true, st);
     if (rc != KFAC_OK) return rc;
     const EpiPlanes make_b = {k[2] * exp2f(-kAExp), k[1], k[0] * exp2f(kAExp), terms,
-                              true};
+                              true, terms == 1};
     rc = plane_launch("ortho A A", poly, make_b, true, st);
     if (rc != KFAC_OK) return rc;
     if (step + 1 < c.steps) {
-      const EpiPlanes make_x = {exp2f(-kAExp), 0.f, 0.f, 2, false};
+      const EpiPlanes make_x = {exp2f(-kAExp), 0.f, 0.f, 2, false, false};
       rc = plane_launch("ortho B X", apply[from], make_x, true, st);
     } else if (c.dtype == KFAC_WIRE_F32) {
       rc = launch_last<N, float>(apply[from], c, st);

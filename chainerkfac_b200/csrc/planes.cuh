@@ -13,8 +13,8 @@
 // out of tensor memory while the MMAs go on in the other one.
 //
 // The tensor core adds with truncation, so a long sum comes out too small by what
-// its number of additions makes: a sum of two-term products is cut every PL_SEGMENT
-// k-blocks and the segments are added in registers, rounded to nearest; within a
+// its number of additions makes: a sum of two-term products is cut every two
+// k-blocks (or each) and the segments are added in registers, rounded to nearest; within a
 // k-block the cross terms, 2^-11 of the others, go first, when the accumulator is
 // small.
 //
@@ -44,10 +44,13 @@ constexpr int PL_BK = 64;                    // k of a stage: 128 bytes of fp16
 constexpr int PL_TERM = PL_ROWS * PL_BK * 2; // bytes of one term of such a part
 constexpr int PL_STAGE_BYTES = 12 * PL_TERM; // 192 KB of stages, 2 to 4 terms each
 constexpr int PL_STAGES_MAX = 6;
-// k-blocks of an accumulator's sum.  4096 x 4096, five steps: 4.9 ms and an error of
-// 0.9e-6 with one, 3.9 ms and 1.9e-6 with two, 3.7 ms and 3.7e-6 with four: of one, a
-// segment is in the tensor cores for less time than it takes to read.
-constexpr int PL_SEGMENT = 2;
+// k-blocks of an accumulator's sum.  4096 x 4096, five steps: 4.3 ms and an error of
+// 1.0e-6 with one, 3.5 ms and 1.9e-6 with two, 3.4 ms and 3.7e-6 with four: of one, a
+// segment is in the tensor cores for less time than it takes to read.  Small tiles'
+// short sums are read in no more time than what is around them: of up to PL_SHORT
+// k-blocks, one (300 x 1000 1.9e-6 and 3.7e-6, both 140 us; of any length 1000 x 1000
+// 253 us and 228, 512 x 4608 237 and 204).
+constexpr int PL_SHORT = 6;
 constexpr int PL_EPI_WARPS = 8;
 constexpr int PL_THREADS = 32 * (4 + PL_EPI_WARPS);
 constexpr int PL_PIECE = 4096;               // bytes of a warp's staging
@@ -75,6 +78,9 @@ struct PlaneFields {
   int a_mn, b_mn;        // k runs down the columns of the operand's planes
   int same;              // A and B are the same operand
   int ta, tb;            // terms of the operands, the same sum in all of a launch
+  int odd;               // k-blocks of an accumulator's sum, less one: 0 or 1 (PL_SHORT)
+  int near;              // 1: A, 2: B, square with one term, has a second one near its
+                         // diagonal: in the rows of a tile, k-blocks of the same numbers
   Planes out;            // of the result (not used by every epilogue)
   Planes add;
   float scale;
@@ -189,14 +195,15 @@ __device__ __forceinline__ void pl_load(unsigned dst, const CUtensorMap* map, in
       : "memory");
 }
 
-// The terms of an operand tile, from (x, y) of its planes.  Rows down the planes: a box
+// `terms` terms of an operand tile from (x, y) of its planes, from the first or the
+// second of them on.  Rows down the planes: a box
 // of 128 rows x 64 k; rows along them (`mn`): two boxes of 64 k x 64 rows.
 template <int G>
 __device__ __forceinline__ void pl_load_terms(unsigned dst, const CUtensorMap* map,
-                                              bool mn, int x, int y, int terms,
-                                              unsigned bar) {
-  pl_load<G>(dst, map, x, y, 0, bar);
-  if (mn) pl_load<G>(dst + PL_TERM / 2, map, x + 64, y, 0, bar);
+                                              bool mn, int x, int y, int from,
+                                              int terms, unsigned bar) {
+  pl_load<G>(dst, map, x, y, from, bar);
+  if (mn) pl_load<G>(dst + PL_TERM / 2, map, x + 64, y, from, bar);
   if (terms < 2) return;
   pl_load<G>(dst + PL_TERM, map, x, y, 1, bar);
   if (mn) pl_load<G>(dst + PL_TERM + PL_TERM / 2, map, x + 64, y, 1, bar);
@@ -435,14 +442,22 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
   constexpr int PARTS = TILE * 512;
   bool apart = true;
   if (S > 1) {
-    const int all = (pl_problem(l, tile0).f.K + PL_BK - 1) / PL_BK;
-    apart = (all + S - 1) / S * stage_bytes <= PL_STAGE_BYTES - PARTS;
+    const PlaneFields& g = pl_problem(l, tile0).f;
+    const int all = (g.K + PL_BK - 1) / PL_BK;
+    const int more = g.near ? (TILE / PL_BK + S - 1) / S : 0;
+    apart = ((all + S - 1) / S + more) * stage_bytes <= PL_STAGE_BYTES - PARTS;
   }
-  // k-blocks of a tile that this pair adds up
-  auto range = [&](const PlaneFields& g, int& kb0, int& nkb) {
+  // k-blocks of a tile that this pair adds up, and with second terms near a diagonal
+  // those behind them: the first from `near0`, each S further
+  auto range = [&](const PlaneFields& g, int m0, int n0, int& kb0, int& nkb, int& near0,
+                   int& more) {
     const int all = (g.K + PL_BK - 1) / PL_BK, each = (all + S - 1) / S;
     kb0 = min(part * each, all);
     nkb = min(each, all - kb0);
+    near0 = (g.near == 1 ? m0 : n0) / PL_BK;
+    const int end = g.near ? min(TILE / PL_BK, all - near0) : 0;
+    more = max(0, (end - part + S - 1) / S);
+    near0 += part;
   };
   int tiles = l.tiles, counted = 0;
   if (l.rows != nullptr) {
@@ -465,9 +480,9 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
       for (int tile = tile0; ok && tile < tiles; tile += step) {
         const PlaneProblem& p = pl_problem(l, tile);
         const PlaneFields g = p.f;
-        int m0, n0, kb0, nkb;
+        int m0, n0, kb0, nkb, near0, more;
         pl_tile_at<G>(g, tile, m0, n0);
-        range(g, kb0, nkb);
+        range(g, m0, n0, kb0, nkb, near0, more);
         const bool share = g.same && m0 == n0, amn = g.a_mn, bmn = g.b_mn;
         const int ta = g.ta, tb = g.tb;
         const unsigned bytes = G * (share ? ta : ta + tb) * PL_TERM;
@@ -481,20 +496,23 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
           // what it wrote is read by the copy engine
           asm volatile("fence.proxy.async.global;" ::: "memory");
         }
-        for (int kb = 0; kb < nkb; ++kb, k += PL_BK) {
+        for (int kb = 0; kb < nkb + more; ++kb, k += PL_BK) {
           if (!mbar_wait_status(&ctl->empty[s], turn, &ctl->abort_flag, status)) {
             ok = false;
             break;
           }
           const unsigned bar = bars + 8 * s, st = stage0 + s * stage_bytes;
+          const bool last = kb >= nkb;         // a second term and a first
           if (side == 0)
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-                         ::"r"(own + 8 * s), "r"(bytes)
+                         ::"r"(own + 8 * s), "r"(last ? 2 * G * PL_TERM : bytes)
                          : "memory");
-          pl_load_terms<G>(st, &p.ma, amn, amn ? ra : k, amn ? k : ra, ta, bar);
+          if (last) k = (near0 + (kb - nkb) * S) * PL_BK;
+          pl_load_terms<G>(st, &p.ma, amn, amn ? ra : k, amn ? k : ra,
+                           last && g.near == 1, last ? 1 : ta, bar);
           if (!share)
             pl_load_terms<G>(st + ta * PL_TERM, &p.mb, bmn, bmn ? rb : k,
-                             bmn ? k : rb, tb, bar);
+                             bmn ? k : rb, last && g.near == 2, last ? 1 : tb, bar);
           if (++s == stages) {
             s = 0;
             turn ^= 1;
@@ -514,9 +532,11 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
       const unsigned stage0 = smem_u32(smem);
       for (int tile = tile0; ok && tile < tiles; tile += step) {
         const PlaneFields g = pl_problem(l, tile).f;
-        int m0, n0, kb0, nkb;
+        int m0, n0, kb0, nkb, near0, more;
         pl_tile_at<G>(g, tile, m0, n0);
-        range(g, kb0, nkb);
+        range(g, m0, n0, kb0, nkb, near0, more);
+        nkb += more;
+        const int full = nkb - more, odd = g.odd;
         const bool share = g.same && m0 == n0;
         const int ta = g.ta, tb = g.tb;
         const bool amn = g.a_mn, bmn = g.b_mn;
@@ -532,7 +552,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
             bmn ? tc_smem_desc_mn(stage_b, PL_TERM / 2) : tc_smem_desc(stage_b);
         unsigned d = 0;
         for (int kb = 0; kb < nkb; ++kb) {
-          const bool fresh = kb == 0 || (cut && kb % PL_SEGMENT == 0);
+          const bool fresh = kb == 0 || (cut && (kb & odd) == 0);
           if (fresh) {
             const int b = seg & 1;
             d = tmem + b * BUFFER;
@@ -551,14 +571,14 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
           const unsigned long long at = (unsigned)(s * stage_bytes) >> 4;
           const unsigned long long a = a0 + at, b = b0 + at;
           unsigned acc = !fresh;
-          if (tb == 2) {
+          if (tb == 2 && kb < full) {
 #pragma unroll
             for (int kk = 0; kk < PL_BK / 16; ++kk) {
               pl_mma<G>(d, a + kk * adv_a, b + lo + kk * adv_b, idesc, acc);
               acc = 1;
             }
           }
-          if (ta == 2) {
+          if (ta == 2 && kb < full) {
 #pragma unroll
             for (int kk = 0; kk < PL_BK / 16; ++kk) {
               pl_mma<G>(d, a + lo + kk * adv_a, b + kk * adv_b, idesc, acc);
@@ -571,7 +591,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
             acc = 1;
           }
           pl_commit<G>(&ctl->empty[s], both);
-          if (kb + 1 == nkb || (cut && (kb + 1) % PL_SEGMENT == 0)) {
+          if (kb + 1 == nkb || (cut && (kb & odd) == odd)) {
             pl_commit<G>(&ctl->accum[seg & 1], both);
             ++seg;
           }
@@ -594,12 +614,13 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
     for (int tile = tile0; ok && tile < tiles; tile += step) {
       PlaneFields g = pl_problem(l, tile).f;
       if (l.rows != nullptr) g.M = counted;
-      int m0, n0, kb0, nkb;
+      int m0, n0, kb0, nkb, near0, more;
       pl_tile_at<G>(g, tile, m0, n0);
-      range(g, kb0, nkb);
+      range(g, m0, n0, kb0, nkb, near0, more);
+      nkb += more;
       t.r0 = m0 + PL_ROWS * side + 32 * q;
       const bool mirror = g.lower && m0 != n0;
-      const int nseg = cut ? (nkb + PL_SEGMENT - 1) / PL_SEGMENT : (nkb > 0 ? 1 : 0);
+      const int nseg = cut ? (nkb + g.odd) >> g.odd : (nkb > 0 ? 1 : 0);
       t.c0 = n0 + COLS * h;
       const auto ahead = epi.begin(g, t);
       float v[COLS];
@@ -756,10 +777,15 @@ inline int plane_map(CUtensorMap* map, const Planes& o, int rows, int cols, bool
 // the 4 n others 1 / 4n, 2 / 4n .. 1: 6 n - 3.5 whole ones.  Errors of orthogonalised
 // 4096 x 4096 and 1024 x 4096 against fp64, with and without:
 // 1.9e-6 and 3.0e-6, 2.3e-6 and 4.0e-6 (fp32 products: 4.3e-6, 3.7e-6).
-inline float plane_gain(int terms, int K) {
-  if (terms < 4) return 1.f;
-  const int n = std::min((K + PL_BK - 1) / PL_BK, PL_SEGMENT);
-  return 1.f + (6 * n - 3.5f) * 0.72f * exp2f(-24);
+// (Parts of a shared sum may be shorter than a segment, and a last one always may.)
+inline float plane_gain(int all, int each, int segment) {
+  float lost = 0.f;
+  for (int left = all; left > 0; left -= each)
+    for (int part = std::min(left, each); part > 0; part -= segment) {
+      const int n = std::min(part, segment);
+      lost += n * (6 * n - 3.5f);
+    }
+  return 1.f + lost / all * 0.72f * exp2f(-24);
 }
 
 // Numbers the tiles of l.p[0 .. l.n), of G blocks each.
@@ -773,7 +799,6 @@ void plane_number_tiles(PlaneLaunch<N>& l, int G) {
     g.tiles_n = tn;
     g.tile_begin = total;
     total += g.lower ? tm * (tm + 1) / 2 : tm * tn;
-    g.gain = plane_gain(g.ta + g.tb, g.K);
   }
   l.tiles = total;
   l.terms = l.n > 0 ? l.p[0].f.ta + l.p[0].f.tb : 0;
@@ -884,6 +909,12 @@ int plane_launch(const char* name, PlaneLaunch<N>& l, const Epi& epi, bool early
   }
   plane_number_tiles(l, best.G);
   l.split = best.split;
+  for (int i = 0; i < l.n; ++i) {
+    PlaneFields& g = l.p[i].f;
+    const int all = (g.K + PL_BK - 1) / PL_BK, each = (all + l.split - 1) / l.split;
+    g.odd = best.G == 1 && each <= PL_SHORT ? 0 : 1;
+    g.gain = g.ta + g.tb < 4 ? 1.f : plane_gain(all, each, g.odd + 1);
+  }
   const int cluster = best.G * l.split;
   const int clusters =
       l.split > 1 ? l.tiles : std::min(l.tiles, rooms[dev][best.G - 1][0]);

@@ -57,10 +57,9 @@ constexpr int PL_PIECE = 4096;               // bytes of a warp's staging
 constexpr int PL_SMEM =
     PL_STAGE_BYTES + PL_EPI_WARPS * PL_PIECE + 1024 /* control */ + 1024 /* align */;
 constexpr int PL_COLS = 512;                 // tensor memory: two accumulators
-// Cycles of an MMA of 128 columns, and what a small tile takes beside its MMAs with a
-// shared sum and without (plane_split).
-constexpr double PL_FEED = 6600;             // bytes a cycle that all SMs get from L2
-constexpr double PL_SMALL_MMA = 85, PL_SMALL_SHARE = 5000, PL_SMALL_END = 5000;
+// Cycles that a small tile takes beside its k-blocks with a shared sum and without
+// (plane_split).
+constexpr double PL_SMALL_SHARE = 5000, PL_SMALL_END = 5000;
 static_assert(256 * 512 <= PL_STAGE_BYTES, "parts of a shared sum");
 
 // A pair of planes.
@@ -806,49 +805,44 @@ void plane_number_tiles(PlaneLaunch<N>& l, int G) {
 
 // Small tiles or large ones, and how many blocks or pairs share one: what a count of
 // cycles comes out least for, with `room[i]` clusters of 2^i of them on the GPU at a
-// time.  A k-block takes an MMA of 128 cycles (small tiles 85 for 64: their operands and
-// the copies into their place want more of the shared memory than its 128 bytes a cycle;
-// 110 of one product) for each 16 k and product of terms; all SMs together get no more
-// than PL_FEED bytes a cycle from L2, and small tiles want twice as many; a tile's start
-// and end 11000 (small 7000; beside the next one's MMAs 2000), with a shared sum 8000
-// (5000) and 500 for each that shares: the parts go through distributed shared memory at
-// 20 bytes a cycle and SM, but each has a part of the epilogue only.  Five steps, us so,
-// with large tiles only, with small ones only: 256 x 512 137, 189, 136; 1000 x 1000
-// 238, 273, 239; 512 x 4608 220, 282, 220; 1024 x 4096 364, 367, 390; 2048 x 2048 556,
-// 679, 590; one matrix of each kind of ResNet-50 450, 509, 458; all 54 of it 1234,
-// 1292, 1273; 8191 x 2047 bf16 856, 856, 1062 (and without PL_FEED 902).
+// time.  A k-block of large tiles takes an MMA of 128 cycles and a little for each 16 k
+// and product of terms.  Small tiles are bound by their shared memory, 128 bytes a cycle:
+// 128 cycles for each term of an operand that is copied in and 256 for each product that
+// reads two, 512, 896 and 1280 with two, three and four terms (counted as 500, 770 and
+// 1040, which fits sums that begin and end: 485 to 1480 were measured).  Their start and end take 7000 cycles (beside the next one's MMAs 2000), a shared sum 5000
+// and 500 for each that shares; large ones' 15000, with a symmetric result, which is
+// stored twice, 19000, a shared sum no less.  Five steps, us so, with large tiles only,
+// with small ones only: 256 x 512 119, 184, 119; 1000 x 1000 228, 269, 228; 512 x 4608
+// 202, 281, 202; 3000 x 1000 365, 347, 404; 2048 x 2048 539, 668, 560; 4096 x 4096 3750,
+// 3720, 4610; one matrix of each kind of ResNet-50 435, 509, 433; all 54 of it 1225,
+// 1305, 1239; bf16 1024 x 4096 262, 274, 233; 8191 x 2047 838, 902, 879.
 struct PlaneShape {
   int G, split;
   double cycles;
 };
 template <int N>
 void plane_split(const PlaneLaunch<N>& l, int G, const int* room, PlaneShape& best) {
-  // of a k-block
-  const double cycles = G == 2           ? (l.terms - 1) * 4 * 132.0
-                        : l.terms == 2 ? 4 * 110.0
-                                       : (l.terms - 1) * 4 * PL_SMALL_MMA;
+  // of a k-block, and of one near a diagonal
+  const double cycles = G == 2 ? (l.terms - 1) * 528.0 : 270.0 * l.terms - 40.0;
+  const double end = l.p[0].f.lower ? 17000 : 13000;
+  const double extra = l.p[0].f.near ? 2 * G * 500.0 : 0;
   for (int i = 0, s = 1; i < 4 && s <= (G == 2 ? 8 : 4); ++i, s *= 2) {
     if (room[i] <= 0) break;
-    const double more = s > 1 ? (G == 2 ? 8000 : PL_SMALL_SHARE) + 500 * s : 2000;
-    double longest = 0, sum = 0, bytes = 0;
+    const double more = s > 1 ? (G == 2 ? end : PL_SMALL_SHARE) + 500 * s : 2000;
+    double longest = 0, sum = 0;
     for (int k = 0; k < l.n; ++k) {
       const int end = k + 1 < l.n ? l.p[k + 1].f.tile_begin : l.tiles;
       const int kb = (l.p[k].f.K + PL_BK - 1) / PL_BK;
-      bytes += (double)kb * (end - l.p[k].f.tile_begin) * l.terms * PL_TERM * G;
-      const double one = (kb + s - 1) / s * cycles + more;
+      const double one = (kb + s - 1) / s * cycles + extra / s + more;
       longest = std::max(longest, one);
       sum += one * (end - l.p[k].f.tile_begin);
     }
-    // (tiles of one size run in whole waves, of different sizes closer together, with
-    // one's start and end beside the other's k-blocks)
+    // (tiles of one size run in whole waves, of different sizes closer together)
     const double waves = (double)l.tiles / room[i];
-    double busy = sum / l.tiles * waves + longest / 2, feed = bytes / PL_FEED;
-    if (l.n == 1) {
-      busy = sum / l.tiles * std::ceil(waves);
-      feed += more * std::ceil(waves);
-    }
-    const double time = std::max(std::max(longest, busy), feed) +
-                        (s > 1 ? 0 : G == 2 ? 9000 : PL_SMALL_END);
+    const double busy = l.n == 1 ? sum / l.tiles * std::ceil(waves)
+                                 : sum / l.tiles * waves + longest / 2;
+    const double time =
+        std::max(longest, busy) + (s > 1 ? 0 : G == 2 ? end : PL_SMALL_END);
     if (best.G == 0 || time < best.cycles) best = {G, s, time};
   }
 }

@@ -10,8 +10,8 @@
 // difference to its values.  The second launch multiplies as many rows as there are,
 // and its epilogue scales and scatters them; the third updates their weights.  (In that
 // epilogue an SM has to store three rows where it now stores one, 32 bytes a cycle:
-// 32000 x 1024 with 12 800 rows took 209 us so, 192 now; 8000 x 256 with 300 rows, four
-// SMs at work, 36 and 29 us.)
+// 32000 x 1024 with 12 800 rows took 209 us so and 192 apart; 8000 x 256 with 300 rows,
+// four SMs at work, 36 and 29.)
 //
 // Bound: HBM, 24 bytes an element (gradient in, kf out, velocity and weight in and
 // out), where the batch reaches few tokens; else the products, three MMAs each.

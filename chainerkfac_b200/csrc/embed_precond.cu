@@ -401,7 +401,6 @@ extern "C" int kfac_precondition_embedding(int64_t vocab, int width, const float
   g = {};
   g.M = (int)vocab;
   g.N = g.K = width;
-  g.ta = g.tb = 2;
   if ((rc = plane_map(&l.p[0].ma, e.rows, (int)vocab, width, false)) != KFAC_OK ||
       (rc = plane_map(&l.p[0].mb, e.g, width, width, false)) != KFAC_OK)
     return rc;

@@ -7,21 +7,18 @@
 // singular vectors.  A and B are symmetric: tiles on and below their diagonals, each
 // stored with its transpose.
 //
-// Operands are planes of fp16 terms (planes.cuh): X 2^13, A 2^12 and B 2^12.  fp32
-// matrices have two terms everywhere.  For 16-bit matrices A and B have one: an error
-// of A or B is relative to a I, of order one, so 2^-12 of it is below the rounding of
-// the result, while an error of X is relative to its largest singular value and grows
-// with the smallest ones (485 times in five steps of the usual coefficients): X keeps
-// two.  Simulated at 512 x 2048 (Gaussian with a part of low rank), error before the
-// last rounding: 1e-3 so, 4e-3 and more with one term of X, 1e-2 with bf16 ones.  Near
-// its diagonal, where its errors are those of whole rows of X, B has two as well.
-// Simulated at 512 x 4608 (Gaussian): 1.6e-3 without, 8e-4 so, and no less with two
-// everywhere.
+// Operands are planes of two fp16 terms (planes.cuh): X 2^13, A 2^12 and B 2^12.  Those
+// of 16-bit matrices too: an error of A or B is relative to a I, of order one, and that
+// of a single term, 2^-12, is as large as the result's own rounding to fp16; of bf16, and
+// with a second term near B's diagonal, it still came to 1.75e-3 where the rounding makes
+// 1.66e-3 (8191 x 2047), and to 2.2e-3 for narrow matrices (33 x 385).  So a 16-bit
+// matrix gives what its values give in fp32, rounded once.  (With one term where errors
+// are damped 8191 x 2047 took 965 us, with two 1713, 4096 x 4096 1850 and 3600.)
 //
 // Entries of 8 and more in X (16 in A and B) are out of range and give NaN; the
 // usual coefficients keep X below 1.3.
 //
-// Bound: the MMAs.  A step takes r^2 c + r^3 + 2 r^2 c flops, thrice with two terms.
+// Bound: the MMAs.  A step takes r^2 c + r^3 + 2 r^2 c flops, each thrice.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -54,7 +51,6 @@ template <int N>
 struct NormLaunch {
   NormJob j[N];
   int n;
-  int dtype;
   double eps;
   double* part;
 };
@@ -176,9 +172,7 @@ ortho_pack_kernel(const __grid_constant__ NormLaunch<N> l) {
 // alpha * sums, with `poly` plus beta * `add` and `diag` on the diagonal, as planes.
 struct EpiPlanes {
   float alpha, beta, diag;
-  int terms;
   bool poly;
-  bool near;             // two terms near the diagonal (in blocks of 256)
   __device__ __forceinline__ NothingAhead begin(const PlaneFields&,
                                                 const PlaneTile&) const {
     return NothingAhead();
@@ -200,7 +194,7 @@ struct EpiPlanes {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           w[term][i] = make_uint4(0, 0, 0, 0);
-          if (term < terms && in && t.r0 + r + 8 * i < g.M)
+          if (in && t.r0 + r + 8 * i < g.M)
             w[term][i] = *reinterpret_cast<const uint4*>(
                 p + (term ? g.add.plane : 0) + 8LL * i * g.add.ld);
         }
@@ -238,8 +232,7 @@ struct EpiPlanes {
             v[i] += diag;
       }
     }
-    const bool both = near && (t.r0 >> 8) == (t.c0 >> 8);
-    pl_store_planes(t, g.out, v, g.M, g.N, both ? 2 : terms, mirror);
+    pl_store_planes(t, g.out, v, g.M, g.N, mirror);
   }
 };
 
@@ -421,7 +414,6 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
               cudaStream_t st) {
   NormLaunch<N> nl;
   nl.n = n;
-  nl.dtype = c.dtype;
   nl.eps = c.eps;
   nl.part = part;
   long long norm_blocks = 0, pack_blocks = 0;
@@ -450,7 +442,6 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
 
   // the three products of a step, with X in either of its places
   PlaneLaunch<N> gram[2], poly, apply[2];
-  const int terms = c.dtype == KFAC_WIRE_F32 ? 2 : 1;   // of A and B
   for (int i = 0; i < n; ++i) {
     const Shape& m = s[i];
     const bool tall = m.rows > m.cols;
@@ -476,8 +467,6 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
       p.M = p.N = r;
       p.K = tall ? m.rows : m.cols;
       p.lower = p.same = 1;
-      // (of X for the product with itself one term, where A has one)
-      p.ta = p.tb = terms;
       p.out = m.a;
       apply[k].p[i].ma = tall ? along[k] : b;
       apply[k].p[i].mb = tall ? b : down[k];
@@ -487,9 +476,6 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
       q.N = m.cols;
       q.K = r;
       q.b_mn = !tall;
-      q.ta = tall ? 2 : terms;
-      q.tb = tall ? terms : 2;
-      q.near = terms == 2 ? 0 : tall ? 2 : 1;
       q.out = m.x[k ^ 1];
     }
     poly.p[i].ma = poly.p[i].mb = a;
@@ -497,7 +483,6 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
     p = g;
     p.M = p.N = p.K = r;
     p.lower = p.same = 1;
-    p.ta = p.tb = terms;
     p.out = m.b;
     p.add = m.a;
   }
@@ -510,15 +495,14 @@ int run_group(const Shape* s, int first, int n, double* part, const Call& c,
   for (int step = 0; step < c.steps; ++step) {
     const float* k = c.coefficients + 3 * step;
     const int from = step & 1;
-    const EpiPlanes make_a = {exp2f(kAExp - 2 * kXExp), 0.f, 0.f, terms, false, false};
+    const EpiPlanes make_a = {exp2f(kAExp - 2 * kXExp), 0.f, 0.f, false};
     rc = plane_launch("ortho X X^T", gram[from], make_a, true, st);
     if (rc != KFAC_OK) return rc;
-    const EpiPlanes make_b = {k[2] * exp2f(-kAExp), k[1], k[0] * exp2f(kAExp), terms,
-                              true, terms == 1};
+    const EpiPlanes make_b = {k[2] * exp2f(-kAExp), k[1], k[0] * exp2f(kAExp), true};
     rc = plane_launch("ortho A A", poly, make_b, true, st);
     if (rc != KFAC_OK) return rc;
     if (step + 1 < c.steps) {
-      const EpiPlanes make_x = {exp2f(-kAExp), 0.f, 0.f, 2, false, false};
+      const EpiPlanes make_x = {exp2f(-kAExp), 0.f, 0.f, false};
       rc = plane_launch("ortho B X", apply[from], make_x, true, st);
     } else if (c.dtype == KFAC_WIRE_F32) {
       rc = launch_last<N, float>(apply[from], c, st);

@@ -62,7 +62,7 @@ __device__ __forceinline__ void os_store16(unsigned addr, uint4 x) {
 // 32 x 32 values (in a PlaneTile's order) as terms: rows r0.., columns c0.. of planes
 // in tiles of 64 columns.
 __device__ __forceinline__ void os_put(unsigned planes, int r0, int c0, int lane,
-                                       const float (&v)[32], int terms) {
+                                       const float (&v)[32]) {
   unsigned hi[16], lo[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) pl_split2(v[2 * i], v[2 * i + 1], hi[i], lo[i]);
@@ -72,17 +72,16 @@ __device__ __forceinline__ void os_put(unsigned planes, int r0, int c0, int lane
   for (int j = 0; j < 4; ++j) {
     const unsigned at = os_at(tile, row, word + j);
     st_matrix(at, hi[2 * j], hi[2 * j + 1], hi[8 + 2 * j], hi[8 + 2 * j + 1]);
-    if (terms == 2)
-      st_matrix(at + OS_PLANE, lo[2 * j], lo[2 * j + 1], lo[8 + 2 * j],
-                lo[8 + 2 * j + 1]);
+    st_matrix(at + OS_PLANE, lo[2 * j], lo[2 * j + 1], lo[8 + 2 * j],
+              lo[8 + 2 * j + 1]);
   }
 }
 
 // v += beta * what is there.
 __device__ __forceinline__ void os_add(unsigned planes, int r0, int c0, int lane,
-                                       float beta, float (&v)[32], int terms) {
+                                       float beta, float (&v)[32]) {
   const unsigned tile = planes + (c0 >> 6) * OS_TILE;
-  for (int term = 0; term < terms; ++term) {
+  for (int term = 0; term < 2; ++term) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       unsigned x[4];
@@ -225,11 +224,6 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
     os_store16(to + OS_PLANE, lo);
   }
 
-  // Two terms of everything, for 16-bit matrices too: of a matrix with few rows the
-  // rounding of A and B to one would be more than the result's own (385 x 33 fp16:
-  // 3.1e-3 of it); 64 x 147 bf16 took 39 us with two and 30 with one, before the sums
-  // of all products of terms shared an accumulator.
-  constexpr int terms = 2;
   const int nk = (r + 15) >> 4, ck = (c + 15) >> 4;
   const int q = warp & 3, h = warp >> 2, r0 = 32 * q;
   unsigned phase = 0;
@@ -289,7 +283,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = ck > 0 ? v[i] * make_a : 0.f;
         if constexpr (!SPLIT) {
-          os_put(A, r0, c0, lane, v, terms);
+          os_put(A, r0, c0, lane, v);
         } else {
           const int unit = q * squares + (c0 >> 5);
           const unsigned to =
@@ -327,10 +321,10 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
             v[4 * i + 3] += y.w;
           }
         }
-        os_put(A, u0, c0, lane, v, terms);
+        os_put(A, u0, c0, lane, v);
         __syncwarp();
         const unsigned tile = A + (c0 >> 6) * OS_TILE;
-        for (int term = 0; term < terms; ++term) {
+        for (int term = 0; term < 2; ++term) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const unsigned at =
@@ -360,7 +354,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
         os_sums(quarter + c0, v);
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] *= cube;
-        os_add(A, r0, c0, lane, k3[1], v, terms);
+        os_add(A, r0, c0, lane, k3[1], v);
         if (c0 == r0) {
           const int d = 2 * (lane & 3) - (lane >> 2);
 #pragma unroll
@@ -371,7 +365,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
               v[i] += diag;
           }
         }
-        os_put(A, r0, c0, lane, v, terms);
+        os_put(A, r0, c0, lane, v);
       }
     }
     // X = B X
@@ -401,7 +395,7 @@ ortho_small_kernel(const __grid_constant__ SmallLaunch l) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] *= make_x;
       if (!last) {
-        os_put(X, r0, c0, lane, v, 2);
+        os_put(X, r0, c0, lane, v);
         continue;
       }
       // out through this warp's 4 KB of what was A

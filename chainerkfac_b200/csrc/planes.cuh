@@ -1,8 +1,7 @@
 // Products of matrices that lie in memory as planes of fp16 terms, x 2^s = hi + lo
 // (row-major, hi in front of lo), C = A B over many problems in one launch, on
-// tcgen05 tensor cores with fp32 accumulators.  An operand gives one term or two;
-// with two on both sides C = hi*hi + (hi*lo + lo*hi), the cross terms in an
-// accumulator of their own: 22 significant bits.
+// tcgen05 tensor cores with fp32 accumulators: C = (hi*lo + lo*hi) + hi*hi in one
+// accumulator, 22 significant bits of every operand.
 //
 // Tiles of 256 x 256 by pairs of CTAs (cta_group::2: each holds 128 rows of A and of
 // C, and half of B's rows), or of 128 x 128 by one CTA where there are few of them,
@@ -13,10 +12,9 @@
 // out of tensor memory while the MMAs go on in the other one.
 //
 // The tensor core adds with truncation, so a long sum comes out too small by what
-// its number of additions makes: a sum of two-term products is cut every two
-// k-blocks (or each) and the segments are added in registers, rounded to nearest; within a
-// k-block the cross terms, 2^-11 of the others, go first, when the accumulator is
-// small.
+// its number of additions makes: a sum is cut every two k-blocks (or each) and
+// the segments are added in registers, rounded to nearest; within a k-block the cross
+// terms, 2^-11 of the others, go first, when the accumulator is small.
 //
 // Launches with fewer tiles than the GPU has room for share the sum of a tile among
 // up to eight pairs (four CTAs) of a cluster, which hand each other their parts through
@@ -42,8 +40,9 @@ static __device__ int g_plane_status = 0;
 constexpr int PL_ROWS = 128;                 // rows of a CTA's part of A, B and C
 constexpr int PL_BK = 64;                    // k of a stage: 128 bytes of fp16
 constexpr int PL_TERM = PL_ROWS * PL_BK * 2; // bytes of one term of such a part
-constexpr int PL_STAGE_BYTES = 12 * PL_TERM; // 192 KB of stages, 2 to 4 terms each
-constexpr int PL_STAGES_MAX = 6;
+constexpr int PL_STAGE = 4 * PL_TERM;        // bytes of a stage: two terms of A and of B
+constexpr int PL_STAGES = 3;
+constexpr int PL_STAGE_BYTES = PL_STAGES * PL_STAGE;
 // k-blocks of an accumulator's sum.  4096 x 4096, five steps: 4.3 ms and an error of
 // 1.0e-6 with one, 3.5 ms and 1.9e-6 with two, 3.4 ms and 3.7e-6 with four: of one, a
 // segment is in the tensor cores for less time than it takes to read.  Small tiles'
@@ -76,10 +75,7 @@ struct PlaneFields {
   int lower;             // square and symmetric: tiles on and below the diagonal
   int a_mn, b_mn;        // k runs down the columns of the operand's planes
   int same;              // A and B are the same operand
-  int ta, tb;            // terms of the operands, the same sum in all of a launch
   int odd;               // k-blocks of an accumulator's sum, less one: 0 or 1 (PL_SHORT)
-  int near;              // 1: A, 2: B, square with one term, has a second one near its
-                         // diagonal: in the rows of a tile, k-blocks of the same numbers
   Planes out;            // of the result (not used by every epilogue)
   Planes add;
   float scale;
@@ -98,15 +94,14 @@ struct PlaneLaunch {
   PlaneProblem p[N];
   int n;
   int tiles;
-  int terms;             // of both operands
   int split;             // CTAs, or pairs of them, that share a tile
   const int* rows;       // the rows of a launch's only problem, where the device counts
                          // them (M is then the most there can be); or null
 };
 
 struct PlaneControl {
-  unsigned long long full[PL_STAGES_MAX];
-  unsigned long long empty[PL_STAGES_MAX];
+  unsigned long long full[PL_STAGES];
+  unsigned long long empty[PL_STAGES];
   unsigned long long accum[2];
   unsigned long long drained[2];
   unsigned tmem_base;
@@ -194,16 +189,13 @@ __device__ __forceinline__ void pl_load(unsigned dst, const CUtensorMap* map, in
       : "memory");
 }
 
-// `terms` terms of an operand tile from (x, y) of its planes, from the first or the
-// second of them on.  Rows down the planes: a box
+// Both terms of an operand tile from (x, y) of its planes.  Rows down the planes: a box
 // of 128 rows x 64 k; rows along them (`mn`): two boxes of 64 k x 64 rows.
 template <int G>
 __device__ __forceinline__ void pl_load_terms(unsigned dst, const CUtensorMap* map,
-                                              bool mn, int x, int y, int from,
-                                              int terms, unsigned bar) {
-  pl_load<G>(dst, map, x, y, from, bar);
-  if (mn) pl_load<G>(dst + PL_TERM / 2, map, x + 64, y, from, bar);
-  if (terms < 2) return;
+                                              bool mn, int x, int y, unsigned bar) {
+  pl_load<G>(dst, map, x, y, 0, bar);
+  if (mn) pl_load<G>(dst + PL_TERM / 2, map, x + 64, y, 0, bar);
   pl_load<G>(dst + PL_TERM, map, x, y, 1, bar);
   if (mn) pl_load<G>(dst + PL_TERM + PL_TERM / 2, map, x + 64, y, 1, bar);
 }
@@ -300,13 +292,13 @@ __device__ __forceinline__ void pl_rows_out(unsigned piece, __half* base, int ld
 // transpose.
 __device__ __forceinline__ void pl_store_planes(const PlaneTile& t, const Planes& o,
                                                 const float (&v)[32], int M, int N,
-                                                int terms, bool mirror) {
+                                                bool mirror) {
   const unsigned piece = smem_u32(t.piece);
   unsigned hi[16], lo[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) pl_split2(v[2 * i], v[2 * i + 1], hi[i], lo[i]);
 #pragma unroll 1
-  for (int term = 0; term < terms; ++term) {
+  for (int term = 0; term < 2; ++term) {
     __half* const base = o.p + (term ? o.plane : 0);
     __syncwarp();
     pl_put_pairs(piece, hi, t.lane);
@@ -397,9 +389,6 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
   PlaneControl* ctl =
       reinterpret_cast<PlaneControl*>(pieces + PL_EPI_WARPS * PL_PIECE);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int stage_bytes = l.terms * PL_TERM;
-  const int stages = PL_STAGE_BYTES / stage_bytes;
-  const bool cut = l.terms == 4;
   const int S = l.split;
   const unsigned rank = cluster_rank(), side = rank % G, first = rank - side;
   const int part = (int)(rank / G);                // of a shared sum
@@ -407,7 +396,7 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
 
   if (warp == 0) {
     if (lane == 0) {
-      for (int s = 0; s < PL_STAGES_MAX; ++s) {
+      for (int s = 0; s < PL_STAGES; ++s) {
         mbar_init(&ctl->full[s], 1);
         mbar_init(&ctl->empty[s], 1);
       }
@@ -443,20 +432,13 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
   if (S > 1) {
     const PlaneFields& g = pl_problem(l, tile0).f;
     const int all = (g.K + PL_BK - 1) / PL_BK;
-    const int more = g.near ? (TILE / PL_BK + S - 1) / S : 0;
-    apart = ((all + S - 1) / S + more) * stage_bytes <= PL_STAGE_BYTES - PARTS;
+    apart = (all + S - 1) / S * PL_STAGE <= PL_STAGE_BYTES - PARTS;
   }
-  // k-blocks of a tile that this pair adds up, and with second terms near a diagonal
-  // those behind them: the first from `near0`, each S further
-  auto range = [&](const PlaneFields& g, int m0, int n0, int& kb0, int& nkb, int& near0,
-                   int& more) {
+  // k-blocks of a tile that this pair adds up
+  auto range = [&](const PlaneFields& g, int& kb0, int& nkb) {
     const int all = (g.K + PL_BK - 1) / PL_BK, each = (all + S - 1) / S;
     kb0 = min(part * each, all);
     nkb = min(each, all - kb0);
-    near0 = (g.near == 1 ? m0 : n0) / PL_BK;
-    const int end = g.near ? min(TILE / PL_BK, all - near0) : 0;
-    more = max(0, (end - part + S - 1) / S);
-    near0 += part;
   };
   int tiles = l.tiles, counted = 0;
   if (l.rows != nullptr) {
@@ -465,9 +447,8 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
     tiles = (counted + TILE - 1) / TILE * l.p[0].f.tiles_n;
   }
   // (The loops over k-blocks carry stages, phases, coordinates and descriptors along:
-  // a k-block of one product is in the tensor cores for 512 cycles, and with divisions
-  // and addresses made anew each of the two threads took 500 and more for one, waits
-  // aside.)
+  // with divisions and addresses made anew each of the two threads took 500 cycles and
+  // more for one, waits aside.)
   if (warp == 0) {
     if (elect_one()) {
       int s = 0;
@@ -479,12 +460,11 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
       for (int tile = tile0; ok && tile < tiles; tile += step) {
         const PlaneProblem& p = pl_problem(l, tile);
         const PlaneFields g = p.f;
-        int m0, n0, kb0, nkb, near0, more;
+        int m0, n0, kb0, nkb;
         pl_tile_at<G>(g, tile, m0, n0);
-        range(g, m0, n0, kb0, nkb, near0, more);
+        range(g, kb0, nkb);
         const bool share = g.same && m0 == n0, amn = g.a_mn, bmn = g.b_mn;
-        const int ta = g.ta, tb = g.tb;
-        const unsigned bytes = G * (share ? ta : ta + tb) * PL_TERM;
+        const unsigned bytes = G * (share ? 2 : 4) * PL_TERM;
         const int ra = m0 + PL_ROWS * side, rb = n0 + PL_ROWS * side;
         int k = kb0 * PL_BK;
         if (!begun) {
@@ -495,24 +475,21 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
           // what it wrote is read by the copy engine
           asm volatile("fence.proxy.async.global;" ::: "memory");
         }
-        for (int kb = 0; kb < nkb + more; ++kb, k += PL_BK) {
+        for (int kb = 0; kb < nkb; ++kb, k += PL_BK) {
           if (!mbar_wait_status(&ctl->empty[s], turn, &ctl->abort_flag, status)) {
             ok = false;
             break;
           }
-          const unsigned bar = bars + 8 * s, st = stage0 + s * stage_bytes;
-          const bool last = kb >= nkb;         // a second term and a first
+          const unsigned bar = bars + 8 * s, st = stage0 + s * PL_STAGE;
           if (side == 0)
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-                         ::"r"(own + 8 * s), "r"(last ? 2 * G * PL_TERM : bytes)
+                         ::"r"(own + 8 * s), "r"(bytes)
                          : "memory");
-          if (last) k = (near0 + (kb - nkb) * S) * PL_BK;
-          pl_load_terms<G>(st, &p.ma, amn, amn ? ra : k, amn ? k : ra,
-                           last && g.near == 1, last ? 1 : ta, bar);
+          pl_load_terms<G>(st, &p.ma, amn, amn ? ra : k, amn ? k : ra, bar);
           if (!share)
-            pl_load_terms<G>(st + ta * PL_TERM, &p.mb, bmn, bmn ? rb : k,
-                             bmn ? k : rb, last && g.near == 2, last ? 1 : tb, bar);
-          if (++s == stages) {
+            pl_load_terms<G>(st + 2 * PL_TERM, &p.mb, bmn, bmn ? rb : k, bmn ? k : rb,
+                             bar);
+          if (++s == PL_STAGES) {
             s = 0;
             turn ^= 1;
           }
@@ -531,27 +508,25 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
       const unsigned stage0 = smem_u32(smem);
       for (int tile = tile0; ok && tile < tiles; tile += step) {
         const PlaneFields g = pl_problem(l, tile).f;
-        int m0, n0, kb0, nkb, near0, more;
+        int m0, n0, kb0, nkb;
         pl_tile_at<G>(g, tile, m0, n0);
-        range(g, m0, n0, kb0, nkb, near0, more);
-        nkb += more;
-        const int full = nkb - more, odd = g.odd;
+        range(g, kb0, nkb);
+        const int odd = g.odd;
         const bool share = g.same && m0 == n0;
-        const int ta = g.ta, tb = g.tb;
         const bool amn = g.a_mn, bmn = g.b_mn;
         const unsigned idesc = pl_desc<G>(amn, bmn);
         // from 16 k to the next (16-byte units)
         const unsigned long long adv_a = (amn ? 2048 : 32) >> 4;
         const unsigned long long adv_b = (bmn ? 2048 : 32) >> 4;
         const unsigned long long lo = PL_TERM >> 4;
-        const unsigned stage_b = share ? stage0 : stage0 + ta * PL_TERM;
+        const unsigned stage_b = share ? stage0 : stage0 + 2 * PL_TERM;
         const unsigned long long a0 =
             amn ? tc_smem_desc_mn(stage0, PL_TERM / 2) : tc_smem_desc(stage0);
         const unsigned long long b0 =
             bmn ? tc_smem_desc_mn(stage_b, PL_TERM / 2) : tc_smem_desc(stage_b);
         unsigned d = 0;
         for (int kb = 0; kb < nkb; ++kb) {
-          const bool fresh = kb == 0 || (cut && (kb & odd) == 0);
+          const bool fresh = (kb & odd) == 0;
           if (fresh) {
             const int b = seg & 1;
             d = tmem + b * BUFFER;
@@ -567,34 +542,26 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const unsigned long long at = (unsigned)(s * stage_bytes) >> 4;
+          const unsigned long long at = (unsigned)(s * PL_STAGE) >> 4;
           const unsigned long long a = a0 + at, b = b0 + at;
           unsigned acc = !fresh;
-          if (tb == 2 && kb < full) {
-#pragma unroll
-            for (int kk = 0; kk < PL_BK / 16; ++kk) {
-              pl_mma<G>(d, a + kk * adv_a, b + lo + kk * adv_b, idesc, acc);
-              acc = 1;
-            }
-          }
-          if (ta == 2 && kb < full) {
-#pragma unroll
-            for (int kk = 0; kk < PL_BK / 16; ++kk) {
-              pl_mma<G>(d, a + lo + kk * adv_a, b + kk * adv_b, idesc, acc);
-              acc = 1;
-            }
-          }
 #pragma unroll
           for (int kk = 0; kk < PL_BK / 16; ++kk) {
-            pl_mma<G>(d, a + kk * adv_a, b + kk * adv_b, idesc, acc);
+            pl_mma<G>(d, a + kk * adv_a, b + lo + kk * adv_b, idesc, acc);
             acc = 1;
           }
+#pragma unroll
+          for (int kk = 0; kk < PL_BK / 16; ++kk)
+            pl_mma<G>(d, a + lo + kk * adv_a, b + kk * adv_b, idesc, 1);
+#pragma unroll
+          for (int kk = 0; kk < PL_BK / 16; ++kk)
+            pl_mma<G>(d, a + kk * adv_a, b + kk * adv_b, idesc, 1);
           pl_commit<G>(&ctl->empty[s], both);
-          if (kb + 1 == nkb || (cut && (kb & odd) == odd)) {
+          if (kb + 1 == nkb || (kb & odd) == odd) {
             pl_commit<G>(&ctl->accum[seg & 1], both);
             ++seg;
           }
-          if (++s == stages) {
+          if (++s == PL_STAGES) {
             s = 0;
             turn ^= 1;
           }
@@ -613,13 +580,12 @@ plane_kernel(const __grid_constant__ PlaneLaunch<N> l,
     for (int tile = tile0; ok && tile < tiles; tile += step) {
       PlaneFields g = pl_problem(l, tile).f;
       if (l.rows != nullptr) g.M = counted;
-      int m0, n0, kb0, nkb, near0, more;
+      int m0, n0, kb0, nkb;
       pl_tile_at<G>(g, tile, m0, n0);
-      range(g, m0, n0, kb0, nkb, near0, more);
-      nkb += more;
+      range(g, kb0, nkb);
       t.r0 = m0 + PL_ROWS * side + 32 * q;
       const bool mirror = g.lower && m0 != n0;
-      const int nseg = cut ? (nkb + g.odd) >> g.odd : (nkb > 0 ? 1 : 0);
+      const int nseg = (nkb + g.odd) >> g.odd;
       t.c0 = n0 + COLS * h;
       const auto ahead = epi.begin(g, t);
       float v[COLS];
@@ -800,32 +766,30 @@ void plane_number_tiles(PlaneLaunch<N>& l, int G) {
     total += g.lower ? tm * (tm + 1) / 2 : tm * tn;
   }
   l.tiles = total;
-  l.terms = l.n > 0 ? l.p[0].f.ta + l.p[0].f.tb : 0;
 }
 
 // Small tiles or large ones, and how many blocks or pairs share one: what a count of
 // cycles comes out least for, with `room[i]` clusters of 2^i of them on the GPU at a
-// time.  A k-block of large tiles takes an MMA of 128 cycles and a little for each 16 k
-// and product of terms.  Small tiles are bound by their shared memory, 128 bytes a cycle:
-// 128 cycles for each term of an operand that is copied in and 256 for each product that
-// reads two, 512, 896 and 1280 with two, three and four terms (counted as 500, 770 and
-// 1040, which fits sums that begin and end: 485 to 1480 were measured).  Their start and end take 7000 cycles (beside the next one's MMAs 2000), a shared sum 5000
+// time.  A k-block of large tiles takes three MMAs of 128 cycles and a little for each
+// 16 k.  Small tiles are bound by their shared memory, 128 bytes a cycle: 128 cycles for
+// each of four terms that are copied in and 256 for each of three products that read
+// two, 1280 (1150 to 1480 were measured; counted as 1040, which fits sums of a few
+// k-blocks that begin and end, and leaves long ones to small tiles too often).  Their
+// start and end take 7000 cycles (beside the next one's MMAs 2000), a shared sum 5000
 // and 500 for each that shares; large ones' 15000, with a symmetric result, which is
 // stored twice, 19000, a shared sum no less.  Five steps, us so, with large tiles only,
 // with small ones only: 256 x 512 119, 184, 119; 1000 x 1000 228, 269, 228; 512 x 4608
 // 202, 281, 202; 3000 x 1000 365, 347, 404; 2048 x 2048 539, 668, 560; 4096 x 4096 3750,
 // 3720, 4610; one matrix of each kind of ResNet-50 435, 509, 433; all 54 of it 1225,
-// 1305, 1239; bf16 1024 x 4096 262, 274, 233; 8191 x 2047 838, 902, 879.
+// 1305, 1239.  (1000 x 8000, 635, is the furthest behind: 580 with large ones only.)
 struct PlaneShape {
   int G, split;
   double cycles;
 };
 template <int N>
 void plane_split(const PlaneLaunch<N>& l, int G, const int* room, PlaneShape& best) {
-  // of a k-block, and of one near a diagonal
-  const double cycles = G == 2 ? (l.terms - 1) * 528.0 : 270.0 * l.terms - 40.0;
+  const double cycles = G == 2 ? 1584 : 1040;          // of a k-block
   const double end = l.p[0].f.lower ? 17000 : 13000;
-  const double extra = l.p[0].f.near ? 2 * G * 500.0 : 0;
   for (int i = 0, s = 1; i < 4 && s <= (G == 2 ? 8 : 4); ++i, s *= 2) {
     if (room[i] <= 0) break;
     const double more = s > 1 ? (G == 2 ? end : PL_SMALL_SHARE) + 500 * s : 2000;
@@ -833,7 +797,7 @@ void plane_split(const PlaneLaunch<N>& l, int G, const int* room, PlaneShape& be
     for (int k = 0; k < l.n; ++k) {
       const int end = k + 1 < l.n ? l.p[k + 1].f.tile_begin : l.tiles;
       const int kb = (l.p[k].f.K + PL_BK - 1) / PL_BK;
-      const double one = (kb + s - 1) / s * cycles + extra / s + more;
+      const double one = (kb + s - 1) / s * cycles + more;
       longest = std::max(longest, one);
       sum += one * (end - l.p[k].f.tile_begin);
     }
@@ -907,7 +871,7 @@ int plane_launch(const char* name, PlaneLaunch<N>& l, const Epi& epi, bool early
     PlaneFields& g = l.p[i].f;
     const int all = (g.K + PL_BK - 1) / PL_BK, each = (all + l.split - 1) / l.split;
     g.odd = best.G == 1 && each <= PL_SHORT ? 0 : 1;
-    g.gain = g.ta + g.tb < 4 ? 1.f : plane_gain(all, each, g.odd + 1);
+    g.gain = plane_gain(all, each, g.odd + 1);
   }
   const int cluster = best.G * l.split;
   const int clusters =

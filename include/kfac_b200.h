@@ -557,11 +557,10 @@ int kfac_token_counts(const void* ids, int id_bytes, int64_t n, int64_t vocab,
  *     param = (1 - lr * decay) * param - lr * scale * X.
  * Either may be NULL, as arrays or element by element; out[i] (or param[i])
  * may be x[i].
- * fp32 products carry 22 bits of their operands; for 16-bit matrices whose
- * sides are both over 128, A carries 11 and so does the polynomial but near
- * its diagonal.  An X with entries
- * of 8 and more, or values that are not finite, give NaN.  Pointer, size and coefficient arrays are host arrays
- * read during the call.  (Matrices with one side of up to 128 and the
+ * Products carry 22 bits of their operands, whatever the type: 16-bit matrices
+ * give what their values give in fp32, rounded once.  An X with entries of 8
+ * and more, or values that are not finite, give NaN.  Pointer, size and
+ * coefficient arrays are host arrays read during the call.  (Matrices with one side of up to 128 and the
  * other of up to 16 x 192 take one launch and no workspace, if all are.) */
 size_t kfac_orthogonalize_workspace_bytes(int count, const int* rows,
                                           const int* cols);

@@ -422,6 +422,7 @@ class KFAC(_base.GradientMethod):
                 continue
             self.fblocks.append(fblock)
         check_embeddings(self.fblocks)
+        self._embedded = embedded_weights(self.target, self.fblocks)
         self._set_low_rank(1, 0, None)
         self.kfhook = KFACHook(self.fblocks)
         self._pre_hooked = False
@@ -608,13 +609,14 @@ class KFAC(_base.GradientMethod):
                 return
         self._accumulated = False
 
+        params = params_to_update(self.target, self._embedded)
         self.reallocate_cleared_grads()
         self.call_hooks('pre')
         self.t += 1
         self.update_kfgrads(self.fblocks)
 
         if not self.only_pic_update_weight:
-            for param in orthogonal.update_together(self.target.params()):
+            for param in orthogonal.update_together(params):
                 param.update()
 
         self.reallocate_cleared_grads()
@@ -1264,6 +1266,11 @@ class DistributedKFAC(KFAC):
         return super(DistributedKFAC, self)._can_fuse(param)
 
 
+def _weight_of(param):
+    """What views of one weight have in common."""
+    return id(getattr(param, '_p', param))
+
+
 def check_embeddings(fblocks):
     """An embedding's weight that another block updates too (an output layer
     that shares it) would be updated twice."""
@@ -1272,13 +1279,53 @@ def check_embeddings(fblocks):
     owner = {}
     for fb in fblocks:
         for param in fb.link.params():
-            other = owner.setdefault(id(getattr(param, '_p', param)), fb)
+            other = owner.setdefault(_weight_of(param), fb)
             if other is not fb and (
                     isinstance(fb, FB.FisherBlockEmbedID) or
                     isinstance(other, FB.FisherBlockEmbedID)):
                 raise ValueError(
                     '%s and %s share a weight: give one of them no block '
                     '(`constructor`)' % (other.linkname, fb.linkname))
+
+
+def embedded_weights(target, fblocks):
+    """The embeddings' weights.  Where one has several names (an output layer
+    shares it), that of the block, or else the first, keeps its rule."""
+    weights = {_weight_of(p) for link in target.links()
+               if isinstance(link, L.EmbedID) for p in link.params()}
+    if weights:
+        keeps = {_weight_of(p): p for fb in fblocks for p in fb.link.params()}
+        for param in target.params():
+            weight = _weight_of(param)
+            if weight in weights and \
+                    keeps.setdefault(weight, param) is not param:
+                param.update_rule = None
+    return weights
+
+
+def params_to_update(target, embedded):
+    """The target's parameters, with the weights of ``embedded`` and those that
+    are orthogonalised once each, however often a module of theirs occurs.
+    Rules for such a weight under several names are refused."""
+    once = embedded.union(
+        _weight_of(p) for p in target.params()
+        if isinstance(p.update_rule, orthogonal.OrthogonalUpdateRule))
+    if not once:
+        return list(target.params())
+    params, ruled = [], {}
+    for name, param in target.namedparams():
+        weight, rule = _weight_of(param), param.update_rule
+        if weight in once and rule is not None and rule.enabled:
+            first, other = ruled.setdefault(weight, (name, param))
+            if other is not param:
+                raise ValueError(
+                    '%s and %s are one weight, and both have an update rule: '
+                    'leave it to one of them (update_rule = None)'
+                    % (first, name))
+            if first != name:
+                continue
+        params.append(param)
+    return params
 
 
 def block_cost(fblock):

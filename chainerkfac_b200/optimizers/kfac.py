@@ -695,7 +695,9 @@ class KFAC(_base.GradientMethod):
 
     def accumulate_grads(self):
         """``kfac.py:286-293``."""
-        params = [p for p in self.target.params() if p.grad is not None]
+        # (a module in several places has one parameter, listed for each)
+        params = [p for p in dict.fromkeys(self.target.params())
+                  if p.grad is not None]
         accs = self._accumulate_group(
             [(p.grad.contiguous(), getattr(p, 'acc_grad', None))
              for p in params])

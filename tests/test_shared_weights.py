@@ -169,3 +169,21 @@ def test_the_weight_after_a_step(block, fused):
     half = 2.0 ** -24
     assert bool((off <= 3 * half * (old.abs() + want.abs())).all())
     assert not torch.equal(old, m[0].weight.detach())
+
+
+def test_gradients_of_a_module_in_two_places_are_accumulated_once(monkeypatch):
+    """acc += grad / 2 in each of two micro-steps."""
+    import chainerkfac_b200 as ck
+    from chainerkfac_b200 import ops
+
+    def axpby(a, xs, b, ys, outs):
+        for x, y, o in zip(xs, ys, outs):
+            o.copy_(a * x + (b * y if b else 0.0))
+    monkeypatch.setattr(ops, 'axpby_group', axpby)
+    e = ck.EmbedID(7, 4)
+    opt = ck.KFAC(constructor=only(), acc_iters=2).setup(Twice(e))
+    for value in (1.0, 3.0):
+        for p in opt.target.params():
+            p.grad = torch.full_like(p.data, value)
+        opt.accumulate()
+    assert torch.equal(e.weight.grad, torch.full((7, 4), 2.0))

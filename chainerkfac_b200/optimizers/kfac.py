@@ -1117,6 +1117,7 @@ class DistributedKFAC(KFAC):
         return self
 
     def update(self, lossfun=None, *args, **kwargs):
+        self._check_rules()
         if lossfun is not None:
             self._forward_backward(
                 lossfun, args, kwargs,
@@ -1142,6 +1143,24 @@ class DistributedKFAC(KFAC):
                 self.reduce_scatter_v_after_backward()
             super(DistributedKFAC, self).update()
             self._real_updates += 1
+
+    def _check_rules(self):
+        """Only the gradients of blocks are exchanged, and by default only their
+        weights updated."""
+        owned = None
+        for param in self.target.params():
+            rule = param.update_rule
+            if isinstance(rule, orthogonal.OrthogonalUpdateRule) and \
+                    rule.enabled:
+                if owned is None:
+                    owned = {p for fb in self.fblocks
+                             for p in fb.link.params()}
+                if param not in owned:
+                    name = [n for n, p in self.target.namedparams()
+                            if p is param][0]
+                    raise ValueError(
+                        '%s has an OrthogonalUpdateRule but no block: its '
+                        'gradient is not exchanged between the ranks' % name)
 
     def _pipeline_ready(self):
         """Whether this step builds, exchanges and averages the factors size

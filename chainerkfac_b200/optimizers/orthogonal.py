@@ -23,7 +23,9 @@ class OrthogonalUpdateRule(_base.UpdateRule):
             p.update_rule = OrthogonalUpdateRule(optimizer.hyperparam)
 
     ``KFAC.update`` orthogonalises the matrices of all such rules together.
-    Float32 weights of two dimensions and more (filters are rows)."""
+    ``DistributedKFAC`` exchanges the gradients of blocks only, and refuses
+    the rule for a parameter without one.  Float32 weights of two dimensions
+    and more (filters are rows)."""
 
     def __init__(self, parent_hyperparam=None, nesterov=True, steps=5,
                  coefficients=ops.NEWTON_SCHULZ, eps=1e-7, decay=0.0,

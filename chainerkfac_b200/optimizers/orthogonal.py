@@ -61,6 +61,12 @@ class OrthogonalUpdateRule(_base.UpdateRule):
         return (h.lr, h.momentum, self.nesterov, self.steps, tuple(c),
                 self.eps, self.decay)
 
+    def prepare(self, param):
+        super(OrthogonalUpdateRule, self).prepare(param)
+        if param._loss_scale is not None and \
+                getattr(param, 'kfgrad', None) is not None:
+            param.kfgrad /= param._loss_scale
+
     def update_core(self, param):
         apply_rules([(self, param)])
 

@@ -1327,10 +1327,15 @@ def embedded_weights(target, fblocks):
 def params_to_update(target, embedded):
     """The target's parameters, with the weights of ``embedded`` and those that
     are orthogonalised once each, however often a module of theirs occurs.
-    Rules for such a weight under several names are refused."""
-    once = embedded.union(
-        _weight_of(p) for p in target.params()
-        if isinstance(p.update_rule, orthogonal.OrthogonalUpdateRule))
+    Rules for such a weight under several names are refused, and weights that
+    cannot be orthogonalised."""
+    once = set(embedded)
+    for param in target.params():
+        rule = param.update_rule
+        if isinstance(rule, orthogonal.OrthogonalUpdateRule):
+            once.add(_weight_of(param))
+            if rule.enabled:
+                rule.check(param)
     if not once:
         return list(target.params())
     params, ruled = [], {}

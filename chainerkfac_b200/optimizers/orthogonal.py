@@ -41,10 +41,20 @@ class OrthogonalUpdateRule(_base.UpdateRule):
         self.decay = decay
         self.scale = scale
 
-    def init_state(self, param):
-        if param.data.dim() < 2:
+    @staticmethod
+    def check(param):
+        """Refuses a weight that the rule's kernels do not take."""
+        w = param.data
+        if w.dim() < 2:
             raise ValueError('%s has %d dimension(s): only matrices can be '
-                             'orthogonalised' % (param.name, param.data.dim()))
+                             'orthogonalised' % (param.name, w.dim()))
+        if w.dtype != torch.float32:
+            raise TypeError('%s is %s: the rule takes float32 weights'
+                            % (param.name, w.dtype))
+        if not w.is_contiguous():
+            raise ValueError('%s must be contiguous' % param.name)
+
+    def init_state(self, param):
         self.state['v'] = torch.zeros_like(param.data)
 
     def _scale_of(self, w):
@@ -62,6 +72,7 @@ class OrthogonalUpdateRule(_base.UpdateRule):
                 self.eps, self.decay)
 
     def prepare(self, param):
+        self.check(param)
         super(OrthogonalUpdateRule, self).prepare(param)
         if param._loss_scale is not None and \
                 getattr(param, 'kfgrad', None) is not None:

@@ -38,3 +38,27 @@ def test_a_blocks_gradient_is_taken_without_the_loss_scale(monkeypatch,
         opt.update()
         assert seen.pop()[0].unique().tolist() == [3.0] and not seen
         assert p.grad.unique().tolist() == [6.0]
+
+
+@pytest.mark.parametrize('model,error,match', [
+    (lambda: nn.Linear(3, 4).half(), TypeError, 'float16'),
+    (lambda: nn.Linear(3, 4).bfloat16(), TypeError, 'bfloat16'),
+    (lambda: nn.Linear(3, 4), ValueError, 'only matrices'),
+    (lambda: nn.Conv2d(3, 4, 3, bias=False).to(
+        memory_format=torch.channels_last), ValueError, 'contiguous')])
+def test_weights_it_cannot_take_are_refused_before_anything_changes(
+        monkeypatch, model, error, match):
+    opt, seen = rules(monkeypatch, model())
+    params = list(opt.target.params())
+    with pytest.raises(error, match=match):
+        opt.update()
+    assert opt.t == 0 and not seen
+    bad = params[-1]
+    with pytest.raises(error, match=match):
+        bad.update()
+    assert all(p.update_rule.t == 0 for p in params)
+    # unless the rule is switched off
+    for p in params:
+        p.update_rule.enabled = False
+    opt.update()
+    assert opt.t == 1 and not seen

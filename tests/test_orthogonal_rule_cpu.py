@@ -41,8 +41,9 @@ def test_a_blocks_gradient_is_taken_without_the_loss_scale(monkeypatch,
 
 
 @pytest.mark.parametrize('model,error,match', [
-    (lambda: nn.Linear(3, 4).half(), TypeError, 'float16'),
-    (lambda: nn.Linear(3, 4).bfloat16(), TypeError, 'bfloat16'),
+    (lambda: nn.Linear(3, 4, bias=False).half(), TypeError, 'float16'),
+    (lambda: nn.Linear(3, 4, bias=False).bfloat16(), TypeError,
+     'bfloat16'),
     (lambda: nn.Linear(3, 4), ValueError, 'only matrices'),
     (lambda: nn.Conv2d(3, 4, 3, bias=False).to(
         memory_format=torch.channels_last), ValueError, 'contiguous')])

@@ -58,6 +58,9 @@ class FisherBlockEmbedID(FisherBlockConnection):
     def compute_A(self, in_data):
         ids = in_data[0].contiguous()
         vocab, link = self.link.W.shape[0], self.link
+        if ids.numel() == 0:
+            raise ValueError('%s: a batch with no tokens has no factors'
+                             % self.linkname)
         if self._A is None or self._A.device != ids.device:
             self._A = torch.empty(vocab, dtype=torch.float32,
                                   device=ids.device)

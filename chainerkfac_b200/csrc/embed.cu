@@ -180,7 +180,7 @@ struct SortCounts {
 };
 
 // Place of each of the thread's keys among its warp's with the same digit, and the
-// warp's counts.  `live`: keys there are (the others behind them).
+// warp's counts.  (Keys behind the end have all bits set and come last.)
 template <int ITEMS>
 __device__ __forceinline__ void rank_keys(SortCounts& s, const int (&key)[ITEMS],
                                           Digit d, int (&rank)[ITEMS]) {

@@ -9,11 +9,12 @@
 //
 // Operands are planes of two fp16 terms (planes.cuh): X 2^13, A 2^12 and B 2^12.  Those
 // of 16-bit matrices too: an error of A or B is relative to a I, of order one, and that
-// of a single term, 2^-12, is as large as the result's own rounding to fp16; of bf16, and
-// with a second term near B's diagonal, it still came to 1.75e-3 where the rounding makes
-// 1.66e-3 (8191 x 2047), and to 2.2e-3 for narrow matrices (33 x 385).  So a 16-bit
-// matrix gives what its values give in fp32, rounded once.  (With one term where errors
-// are damped 8191 x 2047 took 965 us, with two 1713, 4096 x 4096 1850 and 3600.)
+// of a single term, 2^-12, is as large as the result's own rounding to fp16 (512 x 4608:
+// 8.4e-4 where the rounding makes 2.1e-4); of bf16, and with a second term near B's
+// diagonal, it still came to 1.76e-3 where the rounding makes 1.66e-3 (8191 x 2047), and
+// to 2.1e-3 for narrow matrices (33 x 385).  So a 16-bit matrix gives what its values
+// give in fp32, rounded once.  (With one term where errors are damped 8191 x 2047 took
+// 965 us, with two 1713, 4096 x 4096 1850 and 3600.)
 //
 // Entries of 8 and more in X (16 in A and B) are out of range and give NaN; the
 // usual coefficients keep X below 1.3.

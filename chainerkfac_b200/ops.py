@@ -1041,8 +1041,8 @@ def precondition_embedding(G_inv, A, damping, grad, kf=None, param=None,
 
 # -- orthogonalised updates ---------------------------------------------------
 
-# a, b, c of X = a X + (b A + c A A) X: five steps take singular values between
-# 1e-3 and 1 to between 0.7 and 1.2
+# a, b, c of X = a X + (b A + c A A) X (K. Jordan et al., Muon, 2024): five
+# steps take singular values between 1e-3 and 1 to between 0.7 and 1.2
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
 

@@ -1311,7 +1311,7 @@ def check_embeddings(fblocks):
 
 def embedded_weights(target, fblocks):
     """The embeddings' weights.  Where one has several names (an output layer
-    shares it), that of the block, or else the first, keeps its rule."""
+    shares it), only the rule of the block's, or else the first, is enabled."""
     weights = {_weight_of(p) for link in target.links()
                if isinstance(link, L.EmbedID) for p in link.params()}
     if weights:
@@ -1320,7 +1320,7 @@ def embedded_weights(target, fblocks):
             weight = _weight_of(param)
             if weight in weights and \
                     keeps.setdefault(weight, param) is not param:
-                param.update_rule = None
+                param.update_rule.enabled = False
     return weights
 
 
@@ -1346,7 +1346,7 @@ def params_to_update(target, embedded):
             if other is not param:
                 raise ValueError(
                     '%s and %s are one weight, and both have an update rule: '
-                    'leave it to one of them (update_rule = None)'
+                    'leave it to one of them (update_rule.enabled = False)'
                     % (first, name))
             if first != name:
                 continue

@@ -187,3 +187,23 @@ def test_gradients_of_a_module_in_two_places_are_accumulated_once(monkeypatch):
             p.grad = torch.full_like(p.data, value)
         opt.accumulate()
     assert torch.equal(e.weight.grad, torch.full((7, 4), 2.0))
+
+
+def test_every_name_keeps_a_rule(monkeypatch):
+    """Programs go through all parameters' rules (hooks, settings); that of
+    the further name is switched off."""
+    import chainerkfac_b200 as ck
+    m = tied()
+    opt = ck.KFAC(constructor=only('/1')).setup(m)
+    called = []
+    for n, p in opt.target.namedparams():
+        p.update_rule.add_hook(lambda rule, param, n=n: called.append(n),
+                               name='h')
+    assert [p.update_rule.enabled for p in opt.target.params()] == [False, True]
+    assert steps_of(opt, monkeypatch) == [('momentum', m[0].weight.data_ptr())]
+    assert called == ['/1/W']
+    # both switched on: as rules under two names
+    for p in opt.target.params():
+        p.update_rule.enabled = True
+    with pytest.raises(ValueError, match='/0/W and /1/W are one weight'):
+        steps_of(opt, monkeypatch)

@@ -439,8 +439,15 @@ class KFAC(_base.GradientMethod):
         if on and self.fblocks and not self._pre_hooked:
             self._pre_hooked = True
             for fb in self.fblocks:
-                module = getattr(fb.link, 'module', None)
-                if module is not None:
+                # (and the other layers that read an embedding's weight)
+                shared = self._embedded & {_weight_of(p)
+                                           for p in fb.link.params()}
+                links = [fb.link] + [
+                    link for link in self.target.links() if shared and
+                    link is not fb.link and any(_weight_of(p) in shared
+                                                for p in own_params(link))]
+                for module in {getattr(link, 'module', None)
+                               for link in links} - {None}:
                     module.register_forward_pre_hook(
                         lambda m, inp, fb=fb: self._wait_for_block(fb))
 
@@ -1290,6 +1297,11 @@ class DistributedKFAC(KFAC):
 def _weight_of(param):
     """What views of one weight have in common."""
     return id(getattr(param, '_p', param))
+
+
+def own_params(link):
+    """A link's parameters without its children's."""
+    return [getattr(link, attr) for attr in link._params]
 
 
 def check_embeddings(fblocks):

@@ -207,3 +207,25 @@ def test_every_name_keeps_a_rule(monkeypatch):
         p.update_rule.enabled = True
     with pytest.raises(ValueError, match='/0/W and /1/W are one weight'):
         steps_of(opt, monkeypatch)
+
+
+def test_a_tied_layer_waits_for_a_deferred_update(monkeypatch):
+    """With ``defer_join`` a weight may still be being written on a side stream
+    when either of its layers is called."""
+    import chainerkfac_b200 as ck
+    waited = []
+
+    class Stream(object):
+        def wait_event(self, event):
+            waited.append(event)
+    monkeypatch.setattr(torch.cuda, 'current_stream', lambda *a: Stream())
+    for block, at in (('/0', 1), ('/1', 1)):
+        m = tied()
+        opt = ck.KFAC(constructor=only(block)).setup(m)
+        opt.defer_join = True
+        opt._pending_classes = {0: block}
+        opt._block_class = {id(opt.fblocks[0]): 0}
+        m[at](torch.zeros(2, 4))
+        assert waited.pop() == block and not opt._pending_classes
+        m[at](torch.zeros(2, 4))
+        assert not waited
